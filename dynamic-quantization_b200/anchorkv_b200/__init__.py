@@ -11,7 +11,10 @@ kernels behind a C ABI (``include/anchorkv_b200.h``):
   :class:`PagePool` arena, :class:`DeclarativeKVCache` for segment-level
   visibility and eviction;
 * :func:`packed_attention`, the paged split-K decode with an LSE merge
-  (query heads served by :func:`query_head_to_kv_head`'s map), and
+  (query heads served by :func:`query_head_to_kv_head`'s map), optionally through
+  a sliding window with visible first tokens; :func:`chunk_attention` for several
+  query tokens per sequence; :func:`fork_pages` / :func:`compact_pages` for
+  sequences that share pages; and
   :func:`decode_partial_states` / :func:`merge_states` for merging across GPUs;
   ``anchorkv_b200.sharded`` adds the NVLink exchange of one long sequence's
   shards and ``anchorkv_b200.live`` batched Hugging Face decode.
@@ -34,7 +37,9 @@ from .backend import (
     quantize_tensor,
     stack_legacy_cache,
 )
-from .decode import decode_partial_states, merge_states, packed_attention, query_head_to_kv_head
+from .decode import (chunk_attention, decode_partial_states, merge_states, packed_attention,
+                     query_head_to_kv_head)
+from .pages import compact_pages, fork_pages
 from .packed_decode import PagedLayer, QuantizedPage, dense_attention, kl_divergence, pack_page, tensor_bytes
 from .policy import CacheMode, CachePlan, PlannedSegment
 from .pool import PagedBatch, PagePool, pack_dense
@@ -51,5 +56,5 @@ __all__ = [
     "SegmentRecord", "SegmentRole", "decode_partial_states", "dense_attention", "kl_divergence",
     "merge_states", "pack_page", "packed_attention", "quantize_tensor", "stack_legacy_cache",
     "take_device_status", "tensor_bytes", "pack_dense", "shard_range", "gather_states",
-    "sharded_packed_attention", "query_head_to_kv_head",
+    "sharded_packed_attention", "query_head_to_kv_head", "chunk_attention", "compact_pages", "fork_pages",
 ]

@@ -14,7 +14,7 @@ from pathlib import Path
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libanchorkv_b200.so"
 
 OK, ERR_INVALID, ERR_UNSUPPORTED, ERR_CUDA, ERR_SCRATCH = 0, 1, 2, 3, 4
-DEV_BAD_DESCRIPTOR, DEV_TIMEOUT = 1, 2
+DEV_BAD_DESCRIPTOR, DEV_TIMEOUT, DEV_BAD_PARENT = 1, 2, 4
 MODE_SKIP, MODE_INT4, MODE_INT8, MODE_FP16 = 0, 1, 2, 3
 SEM_TENSOR, SEM_PAGE = 0, 1
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
@@ -59,6 +59,15 @@ PROTOTYPES = {
     "akv_packed_attention": (ctypes.c_int, [_c_p, _i64, _c_p, _i64, _c_p, _i32, _c_p, _i64, _i64,
                                             _i32, _i32, _i32, _i32, _i32, _f32, _i32, _c_p, _i64,
                                             _i64, _c_p, _i64, _c_p, _c_p]),
+    "akv_chunk_attention": (ctypes.c_int, [_c_p, _i64, _c_p, _i64, _c_p, _i32, _c_p, _i32, _c_p, _i64, _i64, _i64,
+                                           _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _i32, _i32, _c_p, _i64,
+                                           _i64, _i64, _c_p, _i64, _c_p, _c_p]),
+    "akv_chunk_workspace_bytes": (_i64, [_i32] * 9),
+    "akv_fork_pages": (ctypes.c_int, [_c_p, _i64, _i64, _i32, _i32, _i32, _c_p, _i32, _c_p, _i32, _c_p, _c_p, _c_p,
+                                      _i64, ctypes.c_int, ctypes.c_int, ctypes.c_int, _c_p, _c_p]),
+    "akv_compact_pages": (ctypes.c_int, [_c_p, _i64, _c_p, _c_p, _i64, _c_p, _i64, _c_p, ctypes.c_int, ctypes.c_int,
+                                         ctypes.c_int, _c_p, _i64, _c_p, _c_p]),
+    "akv_compact_workspace_bytes": (_i64, [_i64, _i64, ctypes.c_int, ctypes.c_int, ctypes.c_int]),
     "akv_packed_attention_static": (ctypes.c_int, [_c_p, _i64, _c_p, _i64, _c_p, _i32, _c_p, _i64, _i64,
                                                    _i32, _i32, _i32, _i32, _i32, _f32, _i32, _c_p, _i64,
                                                    _i64, _c_p, _c_p]),
@@ -128,8 +137,30 @@ def stream_of(device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+class _Same:
+    """The device is current already: nothing to enter."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *_):
+        return False
+
+
+_SAME = _Same()
+
+
+def on_device(device):
+    """A context in which ``device`` is the current one, as a launch on its streams needs."""
+    import torch
+
+    index = device.index
+    return _SAME if index is None or index == torch.cuda.current_device() else torch.cuda.device(index)
+
+
 DEV_BITS = {DEV_BAD_DESCRIPTOR: "a page descriptor outside the arena or misaligned (page skipped)",
-            DEV_TIMEOUT: "a bounded wait that gave up (a bulk copy or a peer's exchange flag)"}
+            DEV_TIMEOUT: "a bounded wait that gave up (a bulk copy or a peer's exchange flag)",
+            DEV_BAD_PARENT: "a fork from a parent outside the batch (the child's page table is empty)"}
 
 
 class StatusWord:

@@ -37,6 +37,23 @@ def _workspace_bytes(device: torch.device, *geometry) -> int:
     return nbytes
 
 
+# Pieces a (sequence, KV head, 8 rows) item of a chunk is cut into at least where it
+# has the pages, as packed_attention's default.
+_CHUNK_SPLITS = 4
+
+
+def _chunk_bytes(device: torch.device, *geometry) -> int:
+    """akv_chunk_workspace_bytes for ``geometry`` on ``device``, remembered as _workspace_bytes does."""
+    key = (device.index, "chunk", geometry)
+    nbytes = _workspace_sizes.get(key)
+    if nbytes is None:
+        if len(_workspace_sizes) > 4096:
+            _workspace_sizes.clear()
+        nbytes = _lib.load().akv_chunk_workspace_bytes(*geometry)
+        _workspace_sizes[key] = nbytes
+    return nbytes
+
+
 _MAX_WORKSPACES = 64
 
 
@@ -48,6 +65,10 @@ def _workspace(device: torch.device, nbytes: int, stream: int | None = None) -> 
     per stream forever).  Dropping one is safe: it was allocated on its own
     stream and used only there, so the allocator reuses its memory in that
     stream's order."""
+    if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+        # a captured call's workspace belongs to its graph: one kept here would be
+        # shared by every graph captured on this stream
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
     key = (device.index, torch.cuda.current_stream(device).cuda_stream if stream is None else stream)
     ws = _workspaces.get(key)
     if ws is None or ws.numel() < nbytes:
@@ -117,7 +138,7 @@ def _check_query(query, layer, splits, *, empty_ok: bool) -> int:
     return batch
 
 
-def packed_attention(query, layer, scale, splits=4, *, out=None):
+def packed_attention(query, layer, scale, splits=4, *, out=None, window=None, sinks=0):
     """Attend one query token per sequence over the layer's packed pages.
 
     ``layer``: a PagedLayer, a PagedBatch, or a DeclarativeKVCache of one layer
@@ -129,9 +150,16 @@ def packed_attention(query, layer, scale, splits=4, *, out=None):
     a piece, while the device has resident warps to spare (``0``: every
     resident warp).  Results do not depend on it beyond fp32 rounding.
     ``out``: an optional fp16 CUDA tensor of the query's shape on its device.
+    ``window``: attend only the last ``window`` tokens of each sequence (the
+    query's own among them) and its first ``sinks`` tokens; pages that hold
+    neither are not read.  The layer has to know its token counts (a PagedLayer,
+    ``pack_dense``'s batch, or ``PagedBatch.over(..., tokens=...)``).
     """
     layer = _as_table(layer)
     batch = _check_query(query, layer, splits, empty_ok=False)
+    if window is not None or sinks:
+        _check_window(window, sinks)
+        return _by_position(query, layer, scale, splits, window, sinks, out)
     heads = query.shape[1]
     if out is not None and (out.dtype != torch.float16 or tuple(out.shape) != tuple(query.shape)
                             or out.device != query.device or out.stride(-1) != 1):
@@ -153,6 +181,88 @@ def packed_attention(query, layer, scale, splits=4, *, out=None):
               layer.group, float(scale), splits, out.data_ptr(), out.stride(0), out.stride(1),
               ws.data_ptr(), ws.numel(), _lib.status_ptr(dev), stream)
     return out
+
+
+def _check_window(window, sinks) -> None:
+    if window is not None and window < 1:
+        raise ValueError("window must be at least one token")
+    if sinks < 0 or (sinks and window is None):
+        raise ValueError("sinks must be non-negative and come with a window")
+
+
+def _layer_tokens(layer, batch, device):
+    """(int32 tensor or None, uniform count) of the tokens each sequence holds."""
+    tokens = layer.tokens if isinstance(layer, PagedBatch) else layer.length
+    if tokens is None:
+        raise ValueError("the page table has no token counts (PagedBatch.over(pool, table, tokens=...)), so its "
+                         "columns have no positions")
+    if isinstance(tokens, int):
+        if not 0 <= tokens < 1 << 31:
+            raise ValueError("token counts must be non-negative 32-bit integers")
+        return None, tokens
+    if tokens.dtype != torch.int32 or tuple(tokens.shape) != (batch,) or tokens.device != device \
+            or not tokens.is_contiguous():
+        raise ValueError("tokens must be a contiguous int32 tensor [batch] on the query's device")
+    return tokens, 0
+
+
+def _by_position(query, layer, scale, splits, window, sinks, out):
+    """Attention of query rows that stand at the sequences' last positions."""
+    if out is not None and (out.dtype != torch.float16 or tuple(out.shape) != tuple(query.shape)
+                            or out.device != query.device or out.stride(-1) != 1):
+        raise ValueError("out must be an FP16 tensor of the query's shape on its device, unit stride in head_dim")
+    batch, heads, rows, dim = query.shape
+    dev = query.device
+    arena, arena_bytes, table, seq_blocks, max_blocks = _store_geometry(layer)
+    if arena.device != dev or table.device != dev:
+        raise ValueError("the query and the pages must be on one device")
+    tokens, uniform = _layer_tokens(layer, batch, dev)
+    if out is None:
+        out = torch.empty(query.shape, dtype=query.dtype, device=dev)
+    if out.numel() == 0:
+        return out
+    if query.stride(-1) != 1 or any(s % 8 for s in query.stride()[:-1]) or query.data_ptr() % 16:
+        query = query.contiguous()
+    width = min(window, 1 << 30) if window is not None else 0
+    sinks = min(sinks, 1 << 30)
+    with _lib.on_device(dev):
+        nbytes = _chunk_bytes(dev, batch, rows, heads, layer.heads, dim, max_blocks, width, sinks, splits)
+        if nbytes < 0:
+            raise ValueError('unsupported decode geometry')
+        stream = _lib.stream_of(dev)
+        ws = _workspace(dev, nbytes, stream)
+        _lib.call("akv_chunk_attention", arena.data_ptr(), arena_bytes, table.data_ptr(), table.stride(0),
+                  None if seq_blocks is None else seq_blocks.data_ptr(), max_blocks,
+                  None if tokens is None else tokens.data_ptr(), uniform, query.data_ptr(), *query.stride()[:3],
+                  batch, rows, heads, layer.heads, dim, layer.group, float(scale), width, sinks, splits,
+                  out.data_ptr(), *out.stride()[:3], ws.data_ptr(), ws.numel(), _lib.status_ptr(dev), stream)
+    return out
+
+
+def chunk_attention(query, layer, scale, *, window=None, sinks=0, out=None):
+    """Causal attention of the last tokens of every sequence over its packed pages.
+
+    ``query``: fp16 CUDA ``[batch, Hq, rows, D]``: the last ``rows`` tokens of
+    each sequence, whose keys and values the pages hold already (a prompt's next
+    chunk, or drafted tokens to verify).  Row ``i`` of sequence ``b`` stands at
+    position ``tokens[b] - rows + i`` and attends the resident tokens up to its
+    own.  Sequences shorter than ``rows`` have their padding in front: rows at
+    negative positions, like rows that see no resident token, give zeros.
+    ``layer``: a PagedLayer, or a PagedBatch that knows its token counts.
+    ``window`` / ``sinks``: a row sees its last ``window`` positions (its own
+    among them) and the sequence's first ``sinks``.
+    ``out``: an optional fp16 CUDA tensor of the query's shape, apart from it.
+
+    Values of tokens that no row sees never reach the output, whatever their
+    memory holds; a non-finite value of a token that some row sees may reach the
+    other rows of the call."""
+    layer = _as_table(layer)
+    batched = isinstance(layer, PagedBatch)
+    if query.dim() != 4 or query.shape[0] != (layer.batch if batched else 1) or query.shape[-1] != layer.dim:
+        raise ValueError('query must be [batch, heads, rows, head_dim] for the page table')
+    _check_query(query[:, :, :1], layer, 0, empty_ok=False)
+    _check_window(window, sinks)
+    return _by_position(query, layer, scale, _CHUNK_SPLITS, window, sinks, out)
 
 
 def decode_partial_states(query, layer, scale, splits=0):

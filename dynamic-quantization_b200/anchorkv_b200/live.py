@@ -20,12 +20,19 @@ table per layer that :func:`packed_attention` reads as a ``PagedBatch``:
   counts on the device; a fresh page's descriptors reach the table through
   the same launch (one pinned, non-blocking copy of ``batch`` descriptors);
 * when a page leaves the recent window it is demoted for all sequences at
-  once (``akv_repack_pages``) and its FP16 slots return to the pool.
+  once (``akv_repack_pages``) and its FP16 slots return to the pool;
+* sequences may share pages: ``fork`` gives every new sequence its parent's
+  page tables in one ``akv_fork_pages`` launch over all layers and copies only
+  half-filled last pages (beam search, several samples of one prompt), ``crop``
+  drops the newest tokens (drafts that were not accepted), ``compact`` moves the
+  live pages into an arena of their size.
 
 :func:`batched_live_cache` wraps the store as a transformers ``DynamicCache``
 and :func:`paged_route` registers an attention function that decodes through
 it, so a batched ``model(...)`` step runs two kernel launches per layer for
-attention (decode, merge) plus one append.
+attention (decode, merge) plus one append.  Several query tokens per sequence (a
+prompt's next chunk, drafted tokens) go through :func:`chunk_attention`, and a
+layer's ``sliding_window`` becomes the attention's window.
 
 Model code (``transformers``) is imported lazily: it is needed only when a
 model runs.
@@ -40,7 +47,8 @@ import torch
 
 from . import _lib
 from . import pool as P
-from .decode import packed_attention
+from .decode import chunk_attention, packed_attention
+from .pages import compact_pages, fork_pages
 
 # Name the batched attention function is registered under.
 ROUTE = "anchorkv_b200_batched"
@@ -73,6 +81,9 @@ class PagedKVStore:
         self.pool = P.PagePool(heads, dim, group=group, pages=sizes, device=self.device, zero=False)
         self.tables = torch.zeros((layers, batch, self.capacity), dtype=torch.int64, device=self.device)
         self._desc = np.zeros((layers, batch, self.capacity), np.int64)  # host mirror of the tables
+        # holder[b, j]: the first sequence that names sequence b's page j (b itself where it is
+        # not shared); every layer forks alike, so one map serves them all
+        self._holder = np.repeat(np.arange(batch)[:, None], self.capacity, 1)
         self.lengths = [0] * layers
         self._archived = [-1] * layers
         self.demotions = 0
@@ -88,6 +99,8 @@ class PagedKVStore:
         if tokens > self.capacity * P.BLOCK:
             raise ValueError("cache geometry or capacity exceeded")
         _lib.require_cuda(key, "key")
+        if not any(self.lengths):  # an emptied store: nothing is shared any more
+            self._holder[:] = np.arange(batch)[:, None]
         status, stream = _lib.status_ptr(self.device), _lib.stream_of(self.device)  # raises before any change
         n = -(-tokens // P.BLOCK)
         eligible = tokens // P.BLOCK - self.recent_pages  # complete pages older than the recent window
@@ -139,6 +152,7 @@ class PagedKVStore:
                 new = P.encode_array(np.full(self.batch, _lib.MODE_FP16), np.full(self.batch, take), offs)
                 fresh = P.to_device(new, self.device)
                 self._desc[layer, :, page] = new
+                self._holder[:, page] = np.arange(self.batch)
             else:
                 self._desc[layer, :, page] = (self._desc[layer, :, page] & ~np.int64(15 << 2)) | ((row + take - 1) << 2)
             k, v = key[:, :, done:done + take], value[:, :, done:done + take]
@@ -159,18 +173,142 @@ class PagedKVStore:
             return
         status, stream = _lib.status_ptr(self.device), _lib.stream_of(self.device)  # raises before any change
         self._archived[layer] = max(self._archived[layer], last)
-        src = self._desc[layer][:, pages]  # [batch, n]
+        holder = self._holder[:, pages]
+        own = holder == np.arange(self.batch)[:, None]  # a shared page is repacked once
+        src = self._desc[layer][:, pages][own]
         self.pool.reserve(self.archive_bits, src.size)
         offs = self.pool.alloc_many(self.archive_bits, src.size)
-        dst = P.encode_array(np.full(src.shape, P.BITS_TO_MODE[self.archive_bits]), ((src >> 2) & 15) + 1,
-                             offs.reshape(src.shape))
-        s_dev, d_dev = P.to_device(src.reshape(-1), self.device), P.to_device(dst.reshape(-1), self.device)
+        dst = np.zeros(holder.shape, np.int64)
+        dst[own] = P.encode_array(np.full(src.size, P.BITS_TO_MODE[self.archive_bits]), ((src >> 2) & 15) + 1, offs)
+        packed = dst[own]
+        dst = dst[holder, np.arange(len(pages))]  # every sequence's entry names its holder's page
+        s_dev, d_dev = P.to_device(src, self.device), P.to_device(packed, self.device)
+        entries = d_dev.view(dst.shape) if own.all() else P.to_device(dst, self.device)
         _lib.call("akv_repack_pages", s_dev.data_ptr(), d_dev.data_ptr(), src.size, self.pool.arena.data_ptr(),
                   self.pool.nbytes, self.heads, self.dim, self.group, _lib.SEM_PAGE, status, stream)
-        self.tables[layer].index_copy_(1, P.to_device(pages, self.device), d_dev.view(src.shape))
+        self.tables[layer].index_copy_(1, P.to_device(pages, self.device), entries)
         self._desc[layer][:, pages] = dst
         self.pool.free_many(16, src >> 8)  # stream order: later writes to these slots follow the repack
         self.demotions += src.size
+
+    # ------------------------------------------------- sequences and pages
+    def _even_length(self, what: str) -> int:
+        if len(set(self.lengths)) > 1:
+            raise ValueError(f"{what} works between steps: the layers hold {sorted(set(self.lengths))} tokens")
+        return self.lengths[0]
+
+    def _free_pages(self, sequences: np.ndarray, columns: np.ndarray) -> None:
+        """Return the pages (sequences[i], columns[i]) of every layer to the pool."""
+        desc = self._desc[:, sequences, columns]
+        for bits, mode in P.BITS_TO_MODE.items():
+            self.pool.free_many(bits, desc[(desc & 3) == mode] >> 8)
+
+    def fork(self, parents) -> None:
+        """Make the batch the sequences that continue ``parents`` (indices of
+        present sequences, any number of each; the new batch may be larger or
+        smaller).  A child shares its parent's pages; where several children
+        continue one half-filled page, all but the first get a copy of it (one
+        launch over all layers).  Pages that no child holds return to the pool."""
+        length = self._even_length("fork")
+        index = np.asarray(parents.tolist() if isinstance(parents, torch.Tensor) else parents)
+        if index.ndim != 1 or index.size == 0 or index.dtype.kind not in "iu":
+            raise ValueError("parents must be a non-empty list of sequence indices")
+        if (index < 0).any() or (index >= self.batch).any():
+            raise ValueError(f"parents must lie in [0, {self.batch})")
+        index = index.astype(np.int64)
+        _lib.raise_pending(self.device)  # an earlier kernel's error, before any change
+        children, n = index.size, self.pages()
+        columns = np.arange(n)
+        held = self._holder[index, :n]  # [children, n]: the old holder of each child's page
+        first = np.full((self.batch, n), children)
+        for child in range(children - 1, -1, -1):  # the first child of each old page wins
+            first[held[child], columns] = child
+        holder = np.repeat(np.arange(children)[:, None], self.capacity, 1)
+        holder[:, :n] = first[held, columns]
+        last = length // P.BLOCK
+        copied = np.nonzero(holder[:, last] != np.arange(children))[0] if length % P.BLOCK else np.zeros(0, np.int64)
+        desc = self._desc[:, index]
+        fresh = None
+        if copied.size:
+            self.pool.reserve(16, self.layers * copied.size)
+            offs = self.pool.alloc_many(16, self.layers * copied.size).reshape(self.layers, copied.size)
+            new = np.zeros((self.layers, children), np.int64)
+            new[:, copied] = (offs << 8) | (desc[:, copied, last] & 255)
+            desc[:, copied, last] = new[:, copied]
+            holder[copied, last] = copied
+            fresh = P.to_device(new, self.device)
+        tables = fork_pages(self.pool, self.tables, P.to_device(index, self.device), fresh, tokens=length)
+        gone = (self._holder[:, :n] == np.arange(self.batch)[:, None]) & (first == children)
+        self._free_pages(*np.nonzero(gone))  # stream order: later writes to these slots follow the copies
+        self.batch, self.tables, self._desc, self._holder = children, tables, desc, holder
+
+    def crop(self, tokens: int) -> None:
+        """Keep the first ``tokens`` tokens of every sequence; the pages behind
+        them return to the pool.  A cut inside a page needs that page in FP16 (the
+        next tokens are written there), and gives each sequence its own copy of
+        it where it was shared."""
+        length = self._even_length("crop")
+        if not 0 <= tokens <= length:
+            raise ValueError(f"crop must keep between 0 and {length} tokens")
+        if tokens == length:
+            return
+        _lib.raise_pending(self.device)  # an earlier kernel's error, before any change
+        keep, old = -(-tokens // P.BLOCK), self.pages()
+        own = self._holder == np.arange(self.batch)[:, None]
+        if tokens % P.BLOCK:
+            last = keep - 1
+            if ((self._desc[:, :, last] & 3) != _lib.MODE_FP16).any():
+                raise ValueError(f"token {tokens} lies inside an archived page: crop to a page's first token")
+            self._reopen(last, tokens, own[:, last])
+        sequences, columns = np.nonzero(own[:, keep:old])
+        self._free_pages(sequences, columns + keep)
+        self._desc[:, :, keep:] = 0
+        self._holder[:, keep:] = np.arange(self.batch)[:, None]
+        self.tables[:, :, keep:].zero_()
+        for layer in range(self.layers):
+            self.lengths[layer] = tokens
+            self._archived[layer] = min(self._archived[layer], tokens // P.BLOCK - 1)
+
+    def _reopen(self, page: int, tokens: int, own: np.ndarray) -> None:
+        """Make ``page`` the half-filled last page of every sequence, a copy where it is shared."""
+        fresh = np.zeros((self.layers, self.batch), np.int64)
+        count = (tokens % P.BLOCK - 1) << 2
+        self._desc[:, :, page] = (self._desc[:, :, page] & ~np.int64(15 << 2)) | count
+        self.tables[:, :, page].copy_(P.to_device(self._desc[:, :, page], self.device))
+        if own.all():
+            return
+        copied = np.nonzero(~own)[0]
+        self.pool.reserve(16, self.layers * copied.size)
+        offs = self.pool.alloc_many(16, self.layers * copied.size).reshape(self.layers, copied.size)
+        fresh[:, copied] = (offs << 8) | (self._desc[:, copied, page] & 255)
+        self.tables = fork_pages(self.pool, self.tables, P.to_device(np.arange(self.batch), self.device),
+                                 P.to_device(fresh, self.device), tokens=tokens)
+        self._desc[:, copied, page] = fresh[:, copied]
+        self._holder[copied, page] = copied
+
+    def compact(self) -> int:
+        """Move the live pages into an arena of their number, with FP16 room for
+        every sequence's next page, and drop the old arena.  Returns the bytes by
+        which the arena shrank (negative where that room is more than was free)."""
+        _lib.raise_pending(self.device)  # an earlier kernel's error, before any change
+        n = max(self.pages(layer) for layer in range(self.layers))
+        own = self._holder[:, :n] == np.arange(self.batch)[:, None]
+        modes = self._desc[:, :, :n] & 3
+        live = {bits: int(((modes == mode) & own).sum()) for bits, mode in P.BITS_TO_MODE.items()}
+        room = dict(live)
+        room[16] += self.layers * self.batch
+        into = P.PagePool(self.heads, self.dim, group=self.group, pages=room, device=self.device, zero=False)
+        tables = compact_pages(self.pool, self.tables, into, live)
+        # the same order on the host: pages by first naming, (layer, sequence, column), within a precision
+        desc = np.zeros_like(self._desc)
+        for bits, mode in P.BITS_TO_MODE.items():
+            mine = (modes == mode) & own
+            place = into.base[bits] + np.arange(int(mine.sum()), dtype=np.int64) * into.page_bytes[bits]
+            desc[:, :, :n][mine] = (place << 8) | (self._desc[:, :, :n][mine] & 255)
+        desc[:, :, :n] = desc[:, self._holder[:, :n], np.arange(n)]
+        shrunk = self.pool.nbytes - into.nbytes
+        self.pool, self.tables, self._desc = into, tables, desc
+        return shrunk
 
     # -------------------------------------------------------------- reads
     def pages(self, layer: int = 0) -> int:
@@ -178,7 +316,7 @@ class PagedKVStore:
 
     def batch_view(self, layer: int) -> P.PagedBatch:
         """Layer ``layer``'s page table for :func:`packed_attention` (query ``[batch, Hq, 1, D]``)."""
-        return P.PagedBatch.over(self.pool, self.tables[layer, :, :self.pages(layer)])
+        return P.PagedBatch.over(self.pool, self.tables[layer, :, :self.pages(layer)], tokens=self.lengths[layer])
 
     def bits(self, layer: int = 0) -> np.ndarray:
         """Precision of every page, ``[batch, pages]``."""
@@ -187,10 +325,12 @@ class PagedKVStore:
 
     @property
     def payload_bytes(self) -> int:
-        """Payload + scale bytes of every page (QuantizedPage.nbytes of K and V, packed_decode.py:28-32)."""
+        """Payload + scale bytes of every page, a shared page counted once (QuantizedPage.nbytes of K and V,
+        packed_decode.py:28-32)."""
         total = 0
+        own = self._holder == np.arange(self.batch)[:, None]
         for layer in range(self.layers):
-            bits = self.bits(layer)
+            bits = self.bits(layer)[own[:, :self.pages(layer)]]
             for b_ in (16, 8, 4):
                 per_page = self.heads * (2 * P.BLOCK * self.dim * b_ // 8 +
                                          (0 if b_ == 16 else 4 * P.BLOCK * self.dim // self.group))
@@ -246,6 +386,21 @@ def batched_live_cache(source, *, max_tokens: int, group: int = 64, archive_bits
                 self.store.append(layer_idx, key_states, value_states)
                 return key_states, value_states
 
+            # the model library's names for what the store does (beam search, samples, drafts)
+            def reorder_cache(self, beam_idx):
+                self.store.fork(beam_idx)
+
+            def batch_repeat_interleave(self, repeats):
+                self.store.fork(np.repeat(np.arange(self.store.batch), repeats))
+
+            def batch_select_indices(self, indices):
+                self.store.fork(indices)
+
+            def crop(self, max_length):
+                length = self.store.lengths[0]
+                keep = length + max_length if max_length < 0 else min(max_length, length)
+                self.store.crop(keep)
+
             def report(self):
                 return self.store.report()
 
@@ -260,10 +415,14 @@ def batched_live_cache(source, *, max_tokens: int, group: int = 64, archive_bits
 
 @contextmanager
 def paged_route(model, cache, backend: str = "packed"):
-    """Route ``model``'s attention over ``cache``'s pages (one query token per
-    sequence) for the duration of the block: ``backend="packed"`` decodes with
-    :func:`packed_attention`, ``"dense"`` dequantises the pages and runs SDPA
-    (the reference route's two backends, colab_experiment.py:123-148).  On exit
+    """Route ``model``'s attention over ``cache``'s pages for the duration of the
+    block: ``backend="packed"`` decodes one query token per sequence with
+    :func:`packed_attention` and several with :func:`chunk_attention`,
+    ``"dense"`` dequantises the pages and runs SDPA (the reference route's two
+    backends, colab_experiment.py:123-148).  The step's keys and values are in the
+    pages by then, so tokens that left the recent window within the step are
+    attended at the archive precision.  A layer with a ``sliding_window`` attends
+    that many last positions.  On exit
     the model's attention implementation is restored and the registry entry
     points back at SDPA, so it keeps no reference to the cache."""
     from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
@@ -274,15 +433,23 @@ def paged_route(model, cache, backend: str = "packed"):
     store = cache.store
 
     def attention(module, query, key, value, attention_mask, scaling, **kwargs):
-        if query.shape[2] != 1:
-            raise ValueError("the paged route decodes one token per sequence; prefill with the stock model")
-        if backend == "packed":
-            out = packed_attention(query, store.batch_view(module.layer_idx), scaling)
-        else:
+        view = store.batch_view(module.layer_idx)
+        window = kwargs.get("sliding_window")
+        if backend == "dense":
             k, v = store.dense(module.layer_idx)
             g = query.shape[1] // k.shape[1]
+            rows, length = query.shape[2], k.shape[2]
+            mask = None
+            if rows > 1 or window is not None:
+                at = torch.arange(length - rows, length, device=query.device)[:, None]
+                pos = torch.arange(length, device=query.device)
+                mask = (pos <= at) & (pos > at - (window or length))
             out = torch.nn.functional.scaled_dot_product_attention(
-                query, k.repeat_interleave(g, 1), v.repeat_interleave(g, 1), scale=scaling)
+                query, k.repeat_interleave(g, 1), v.repeat_interleave(g, 1), attn_mask=mask, scale=scaling)
+        elif query.shape[2] == 1:
+            out = packed_attention(query, view, scaling, window=window)
+        else:
+            out = chunk_attention(query, view, scaling, window=window)
         return out.transpose(1, 2), None
 
     previous = model.config._attn_implementation

@@ -117,6 +117,68 @@ def group_ok(dim: int, group: int) -> bool:
     return group in (32, 64, 128, BLOCK * dim)
 
 
+class _FreeSlots:
+    """Free byte offsets of one size class: a stack of returned slots over runs of
+    never used ones (first, step, count), so a pool of any size is set up at
+    once and slots move by whole arrays.  Slots come back last in, first out;
+    then the runs in ascending order."""
+
+    __slots__ = ("_stack", "_top", "_runs", "_in_runs")
+
+    def __init__(self):
+        self._stack, self._top = np.zeros(0, np.int64), 0
+        self._runs, self._in_runs = [], 0
+
+    def __len__(self) -> int:
+        return self._top + self._in_runs
+
+    def add_run(self, first: int, step: int, count: int) -> None:
+        if count > 0:
+            self._runs.append([first, step, count])
+            self._in_runs += count
+
+    def take(self, n: int) -> np.ndarray:
+        out = np.empty(n, np.int64)
+        got = min(n, self._top)
+        out[:got] = self._stack[self._top - got:self._top][::-1]
+        self._top -= got
+        while got < n:
+            run = self._runs[0]
+            k = min(n - got, run[2])
+            out[got:got + k] = run[0] + run[1] * np.arange(k, dtype=np.int64)
+            run[0] += run[1] * k
+            run[2] -= k
+            if run[2] == 0:
+                self._runs.pop(0)
+            got += k
+            self._in_runs -= k
+        return out
+
+    def untouched(self, first: int, count: int) -> bool:
+        """Whether every slot of a class of ``count`` from byte ``first`` is free, in ascending order."""
+        if count == 0:
+            return len(self) == 0
+        return self._top == 0 and len(self._runs) == 1 and self._runs[0][0] == first and self._runs[0][2] == count
+
+    def skip(self, n: int) -> None:
+        """Take the first ``n`` slots of an untouched class (no array of them is made)."""
+        if n:
+            run = self._runs[0]
+            run[0], run[2] = run[0] + run[1] * n, run[2] - n
+            self._in_runs -= n
+            if run[2] == 0:
+                self._runs.pop()
+
+    def give(self, offsets: np.ndarray) -> None:
+        need = self._top + offsets.size
+        if need > self._stack.size:
+            grown = np.empty(max(need, 2 * self._stack.size), np.int64)
+            grown[:self._top] = self._stack[:self._top]
+            self._stack = grown
+        self._stack[self._top:need] = offsets
+        self._top = need
+
+
 class PagePool:
     """An arena of page slots in three size classes (FP16 / INT8 / INT4).
 
@@ -125,40 +187,69 @@ class PagePool:
     random physical placement of a long-lived shared pool).
     """
 
+    fixed = False  # over(): the arena is the caller's and never grows
+
     def __init__(self, heads: int, dim: int, *, group: int = 64, pages: dict | None = None,
                  device="cuda", shuffle_seed: int | None = None, zero: bool = True):
         if dim not in (64, 128):
             raise ValueError("supported geometry: head dim 64 or 128")
         if not group_ok(dim, group):
             raise ValueError(f"supported scale groups for head dim {dim}: 32, 64, 128, {BLOCK * dim}")
-        self.heads, self.dim, self.group = heads, dim, group
         self.device = torch.device(device)
+        self._lay_out(heads, dim, group, pages)
+        if shuffle_seed is not None:
+            rng = np.random.default_rng(shuffle_seed)
+            for bits in (16, 8, 4):
+                slots = np.arange(self.capacity[bits], dtype=np.int64)
+                rng.shuffle(slots)
+                self._free[bits] = _FreeSlots()
+                # the stack gives its last entry first: reverse so slot order is allocation order
+                self._free[bits].give((self.base[bits] + slots * self.page_bytes[bits])[::-1])
+        alloc = torch.zeros if zero else torch.empty
+        self.arena = alloc(self.nbytes, dtype=torch.uint8, device=self.device)
+
+    def _lay_out(self, heads: int, dim: int, group: int, pages: dict | None) -> None:
+        self.heads, self.dim, self.group = heads, dim, group
         pages = dict(pages or {})
         self.page_bytes = {b: heads * record_bytes(dim, group, b) for b in (4, 8, 16)}
         self.base, self.capacity, self._free = {}, {}, {}
         cursor = 0
-        rng = np.random.default_rng(shuffle_seed) if shuffle_seed is not None else None
         for bits in (16, 8, 4):
             n = int(pages.get(bits, 0))
             self.base[bits] = cursor
             self.capacity[bits] = n
-            slots = np.arange(n, dtype=np.int64)
-            if rng is not None:
-                rng.shuffle(slots)
-            # pop() takes from the end: reverse so slot order is allocation order.
-            self._free[bits] = list((cursor + slots * self.page_bytes[bits])[::-1])
+            self._free[bits] = _FreeSlots()
+            self._free[bits].add_run(cursor, self.page_bytes[bits], n)
             cursor += n * self.page_bytes[bits]
         self.nbytes = max(cursor, 16)
-        alloc = torch.zeros if zero else torch.empty
-        self.arena = alloc(self.nbytes, dtype=torch.uint8, device=self.device)
+
+    @classmethod
+    def over(cls, arena: torch.Tensor, heads: int, dim: int, *, group: int = 64, pages: dict | None = None) -> "PagePool":
+        """A pool over a caller's arena: a contiguous, 16-byte aligned uint8 CUDA tensor.
+
+        ``pages`` lays its slots out as the constructor does (FP16, then INT8,
+        then INT4 slots, all free); without it the pool only names the memory
+        that existing tables point into, and has no slots of its own.  The arena
+        never grows: a request for more slots raises MemoryError."""
+        if dim not in (64, 128) or not group_ok(dim, group):
+            raise ValueError(f"supported geometry: head dim 64 or 128, scale groups 32, 64, 128, {BLOCK * dim}")
+        if arena.dtype != torch.uint8 or arena.dim() != 1 or not arena.is_contiguous() or arena.data_ptr() % 16:
+            raise ValueError("the arena must be a contiguous, 16-byte aligned one-dimensional uint8 tensor")
+        pool = cls.__new__(cls)
+        pool.device, pool.fixed = arena.device, True
+        pool._lay_out(heads, dim, group, pages)
+        if pages and pool.nbytes > arena.numel():
+            raise ValueError(f"{pool.nbytes} bytes of page slots do not fit an arena of {arena.numel()}")
+        pool.nbytes, pool.arena = arena.numel(), arena
+        return pool
 
     def free_slots(self, bits: int) -> int:
         return len(self._free[bits])
 
     def alloc(self, bits: int) -> int:
-        if not self._free[bits]:
+        if not len(self._free[bits]):
             raise MemoryError(f"page pool has no free {bits}-bit page slots")
-        return int(self._free[bits].pop())
+        return int(self._free[bits].take(1)[0])
 
     def check_free(self, bits: int, n: int) -> None:
         """Raise MemoryError unless ``n`` slots of ``bits`` are free (nothing changes)."""
@@ -167,17 +258,23 @@ class PagePool:
 
     def alloc_many(self, bits: int, n: int) -> np.ndarray:
         self.check_free(bits, n)
-        if n == 0:
-            return np.zeros(0, np.int64)
-        out = np.array(self._free[bits][-n:][::-1], dtype=np.int64)
-        del self._free[bits][-n:]
-        return out
+        return self._free[bits].take(n)
 
     def free(self, bits: int, offset: int) -> None:
-        self._free[bits].append(int(offset))
+        self._free[bits].give(np.array([offset], np.int64))
 
     def free_many(self, bits: int, offsets) -> None:
-        self._free[bits].extend(int(o) for o in np.asarray(offsets).reshape(-1))
+        self._free[bits].give(np.asarray(offsets, np.int64).reshape(-1))
+
+    @property
+    def untouched(self) -> bool:
+        """Whether no slot was ever taken and the pool never grew or was shuffled: its slots are then handed
+        out in ascending order from each class's base (the order compact_pages fills them in)."""
+        return all(self._free[b].untouched(self.base[b], self.capacity[b]) for b in (4, 8, 16))
+
+    def claim(self, bits: int, n: int) -> None:
+        """Take the first ``n`` slots of an untouched pool's class without naming them."""
+        self._free[bits].skip(n)
 
     def reserve(self, bits: int, n: int) -> None:
         """Make at least ``n`` slots of ``bits`` free, growing the arena if needed.
@@ -190,6 +287,8 @@ class PagePool:
         short = n - len(self._free[bits])
         if short <= 0:
             return
+        if self.fixed:
+            self.check_free(bits, n)  # raises: the arena is the caller's
         extra = max(short, self.capacity[bits], 64)
         start = self.nbytes
         old = self.arena
@@ -197,8 +296,7 @@ class PagePool:
         self.arena = torch.empty(self.nbytes, dtype=torch.uint8, device=self.device)
         self.arena[:start].copy_(old[:start])
         self.arena[start:].zero_()
-        new = start + np.arange(extra, dtype=np.int64) * self.page_bytes[bits]
-        self._free[bits] = list(new[::-1]) + self._free[bits]  # old free slots are taken first
+        self._free[bits].add_run(start, self.page_bytes[bits], extra)  # old free slots are taken first
         self.capacity[bits] += extra
 
     def page_view(self, offset: int, bits: int) -> torch.Tensor:
@@ -213,7 +311,14 @@ class PagedBatch:
     ``table[b, j]`` is the descriptor of page ``j`` of sequence ``b``;
     ``seq_blocks[b]`` the number of pages sequence ``b`` uses.  Skip entries
     (evicted or invisible pages) are never read by the decode kernel.
+
+    ``tokens`` (an int32 tensor ``[batch]`` on the pool's device, one int for
+    all sequences, or None where they are not known) is how many tokens each
+    sequence holds, evicted ones included: column ``j`` holds positions ``16 j``
+    to ``16 j + 15``.  Attention that goes by position needs it.
     """
+
+    tokens = None
 
     def __init__(self, pool: PagePool, batch: int, max_blocks: int):
         self.pool = pool
@@ -222,11 +327,12 @@ class PagedBatch:
         self.seq_blocks = torch.full((batch,), max_blocks, dtype=torch.int32, device=pool.device)
 
     @classmethod
-    def over(cls, pool: PagePool, table: torch.Tensor) -> "PagedBatch":
+    def over(cls, pool: PagePool, table: torch.Tensor, *, tokens=None) -> "PagedBatch":
         """A batch over an existing ``[batch, max_blocks]`` descriptor table (a
-        view, no allocation); every sequence uses all ``max_blocks`` entries."""
+        view, no allocation); every sequence uses all ``max_blocks`` entries, or
+        those of its ``tokens`` where attention goes by position."""
         view = cls.__new__(cls)
-        view.pool, view.table, view.seq_blocks = pool, table, None
+        view.pool, view.table, view.seq_blocks, view.tokens = pool, table, None, tokens
         view.batch, view.max_blocks = int(table.shape[0]), int(table.shape[1])
         return view
 
@@ -310,4 +416,5 @@ def pack_dense(pool: PagePool, key: torch.Tensor, value: torch.Tensor, block_bit
     out.table.copy_(torch.from_numpy(desc))
     out.seq_blocks.copy_(torch.from_numpy(blocks_used.astype(np.int32)))
     out.lengths = lengths
+    out.tokens = torch.from_numpy(lengths.astype(np.int32)).to(dev)
     return out

@@ -457,12 +457,6 @@ __global__ void __launch_bounds__(256) dequantize_vec_kernel(const uint8_t *__re
   }
 }
 
-// Descriptor check shared by the page kernels.
-__device__ __forceinline__ bool page_in_arena(int64_t desc, int64_t page_bytes, int64_t arena_bytes) {
-  const int64_t off = desc_offset(desc);
-  return (off & 15) == 0 && off >= 0 && off + page_bytes <= arena_bytes;
-}
-
 // Pack (SRC_RECORD = false: dense fp16 source) or repack (SRC_RECORD = true:
 // source records in the arena) one slab per warp.  A repack holds both the
 // source record's reads and the destination's stores, so it runs 2 CTAs per

@@ -40,6 +40,12 @@ __host__ __device__ inline int64_t record_bytes(int D, int group, int mode) {
   return (b + 15) & ~(int64_t)15;
 }
 
+// Descriptor check shared by the page kernels.
+__device__ __forceinline__ bool page_in_arena(int64_t desc, int64_t page_bytes, int64_t arena_bytes) {
+  const int64_t off = desc_offset(desc);
+  return (off & 15) == 0 && off >= 0 && off + page_bytes <= arena_bytes;
+}
+
 // V payload byte order.  The 16-byte units of a V payload are permuted inside
 // each 128-byte line: unit u of the line holding token row r is stored at
 // u ^ S(r), with S chosen per row width (D * bits / 8 bytes) so that the
@@ -198,6 +204,25 @@ __device__ __forceinline__ uint32_t int8_to_f16x2(uint32_t w) {
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void allow_dependents_launch() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+// Launch with programmatic stream serialization: the kernel may begin while its
+// predecessor in the stream finishes (it calls grid_dependency_wait() before
+// touching memory the predecessor may write or read).
+template <typename... Params, typename... Args>
+static cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem,
+                                    cudaStream_t s, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 // --------------------------------------------------------- PTX: tensor cores

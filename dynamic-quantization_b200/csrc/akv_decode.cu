@@ -67,7 +67,8 @@ struct DecodeTraits {
   static constexpr int DV = D / 8;      // V dims a lane owns per row
   static constexpr int kTiles = D / 16;
   // A warp's shared memory: its ring, then its slot barriers and records.
-  static constexpr int kWarpBytes = kRing + kSlots * (8 + 4 + 4 + 4);
+  // A multi-row decode's slots also hold their pages' table columns.
+  static constexpr int kWarpBytes = kRing + kSlots * (8 + 4 + 4 + 4 + 8);
   static constexpr int kSmemMax = kMaxWarps * kWarpBytes;
   static_assert(kRing % 16 == 0 && kWarpBytes % 16 == 0, "rings stay 16-byte aligned");
   static_assert(kRing >= 4 * kBlock * D, "a ring must hold one FP16 record");
@@ -115,6 +116,13 @@ struct DecodeParams {
   int32_t batch, q_heads, kv_heads, gqa, qgroups, items, log2_group;
   int32_t warps, range, smax, slot_heads;
   FastDiv fd_mb, fd_ipb, fd_qgroups;  // max_blocks, kv_heads * qgroups, qgroups
+  // Multi-row decode (RowsTag): `rows` query tokens per sequence, the last of
+  // its `tokens` (or uniform_tokens), gqa counting rows x query heads per KV
+  // head; max_blocks is then the columns an item may see (visible_columns).
+  const int32_t *tokens;
+  int32_t uniform_tokens, rows, heads_per_kv, columns, window, sinks, lead;
+  int64_t q_ts;
+  FastDiv fd_hpk;
   float scale_log2;
   int32_t *header;
   float *partials;
@@ -321,16 +329,39 @@ struct SoftmaxState {
   float m0, m1, l0, l1;  // heads 2t4, 2t4+1: running max (base 2) and this lane's sum
 };
 
+// What the rows of one item of a multi-row decode see: row n (lane rows 2t4,
+// 2t4+1 here) stands at token position at0 / at1 and sees positions up to its
+// own that lie less than `window` tokens back or below `sinks`; at_lo and at_hi
+// are the item's lowest and highest row positions.
+struct RowView {
+  int at0, at1, at_lo, at_hi, window, sinks;
+  __device__ __forceinline__ bool sees(int at, int pos) const {
+    return pos <= at && (pos > at - window || pos < sinks);
+  }
+  // Whether some row of the item may see `pos` (exact for one row; a superset
+  // of the union of the rows' sets otherwise).
+  __device__ __forceinline__ bool any(int pos) const {
+    return pos <= at_hi && (pos > at_lo - window || pos < sinks);
+  }
+  // Whether every row of the item sees all 16 tokens of page column `col`.
+  __device__ __forceinline__ bool whole_page(int col) const {
+    const int p0 = kBlock * col, p1 = p0 + kBlock - 1;
+    return p1 <= at_lo && (p0 > at_hi - window || p1 < sinks);
+  }
+};
+
 // Online softmax step over one or two pages of one item (fp32, base 2).
 // Returns the fp16 P fragments for P.V.  Scores are scaled before the max, so
 // any sign of the softmax scale works.  The running max moves only when a score
 // exceeds it by more than 2^8 (P <= 2^8 stays exact enough in fp16 and most
 // pages need no reduction).  With NP = 2 the second page is skipped when `two`
 // is false.
-template <int D, int NP>
+// ROWS: `part[r]` says that some row does not see all of page r (column col[r]).
+template <int D, int NP, bool ROWS>
 __device__ __forceinline__ void pages_softmax(float (&s)[NP][4], const int (&ntok)[NP], bool two,
                                               int gid, float scale_log2, SoftmaxState &st,
-                                              float (&o)[D / 16][4], uint32_t (&b)[NP][2]) {
+                                              float (&o)[D / 16][4], uint32_t (&b)[NP][2],
+                                              const bool (&part)[NP], const int (&col)[NP], const RowView &view) {
   constexpr float slack = 8.f;
   constexpr float kNegInf = -INFINITY;
   float x[NP][4];
@@ -343,6 +374,15 @@ __device__ __forceinline__ void pages_softmax(float (&s)[NP][4], const int (&nto
       if (gid >= ntok[r]) x[r][0] = x[r][1] = kNegInf;
       if (gid + 8 >= ntok[r]) x[r][2] = x[r][3] = kNegInf;
     }
+    if constexpr (ROWS) {
+      if (part[r]) {
+        const int pos = kBlock * col[r] + gid;
+        if (!view.sees(view.at0, pos)) x[r][0] = kNegInf;
+        if (!view.sees(view.at1, pos)) x[r][1] = kNegInf;
+        if (!view.sees(view.at0, pos + 8)) x[r][2] = kNegInf;
+        if (!view.sees(view.at1, pos + 8)) x[r][3] = kNegInf;
+      }
+    }
     mx0 = fmaxf(mx0, fmaxf(x[r][0], x[r][2]));
     mx1 = fmaxf(mx1, fmaxf(x[r][1], x[r][3]));
   }
@@ -354,7 +394,11 @@ __device__ __forceinline__ void pages_softmax(float (&s)[NP][4], const int (&nto
       mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, off));
     }
     const float n0 = fmaxf(st.m0, mx0), n1 = fmaxf(st.m1, mx1);
-    const float a0 = ex2(st.m0 - n0), a1 = ex2(st.m1 - n1);
+    float a0 = ex2(st.m0 - n0), a1 = ex2(st.m1 - n1);
+    if constexpr (ROWS) {  // a row that has seen nothing yet has both maxima at -inf
+      if (n0 == kNegInf) a0 = 1.f;
+      if (n1 == kNegInf) a1 = 1.f;
+    }
     st.l0 *= a0, st.l1 *= a1;
 #pragma unroll
     for (int m = 0; m < D / 16; ++m) o[m][0] *= a0, o[m][1] *= a1, o[m][2] *= a0, o[m][3] *= a1;
@@ -363,8 +407,10 @@ __device__ __forceinline__ void pages_softmax(float (&s)[NP][4], const int (&nto
 #pragma unroll
   for (int r = 0; r < NP; ++r) {
     if (r > 0 && !two) break;
-    const float p0 = ex2(x[r][0] - st.m0), p1 = ex2(x[r][1] - st.m1);
-    const float p2 = ex2(x[r][2] - st.m0), p3 = ex2(x[r][3] - st.m1);
+    // A row that has seen nothing weighs its tokens against 0, not against -inf.
+    const float m0 = ROWS && st.m0 == kNegInf ? 0.f : st.m0, m1 = ROWS && st.m1 == kNegInf ? 0.f : st.m1;
+    const float p0 = ex2(x[r][0] - m0), p1 = ex2(x[r][1] - m1);
+    const float p2 = ex2(x[r][2] - m0), p3 = ex2(x[r][3] - m1);
     st.l0 += p0 + p2, st.l1 += p1 + p3;
     b[r][0] = movmatrix_trans(pack_f16x2(p0, p1));
     b[r][1] = movmatrix_trans(pack_f16x2(p2, p3));
@@ -382,16 +428,37 @@ __device__ __forceinline__ void zero_tail(uint8_t *rec, int ntok, int lane) {
   constexpr int rowB = D * mode_bits(MODE) / 8;
   for (int off = ((ntok * rowB) & ~127) + 4 * lane; off < PB; off += 128)
     if ((int)v_swizzle(D, MODE, off) >= ntok * rowB) *reinterpret_cast<uint32_t *>(rec + PB + off) = 0u;
+  fence_proxy_async_smem();  // the next copy into this ring space comes after these writes
+}
+
+// Zero the V rows of page column `col` that no row of the item sees (or that lie
+// past the valid count), for the same reason.
+template <int D, int MODE>
+__device__ __forceinline__ void zero_unseen(uint8_t *rec, int ntok, int col, const RowView &view, int lane) {
+  constexpr int PB = kBlock * D * mode_bits(MODE) / 8;
+  constexpr int rowB = D * mode_bits(MODE) / 8;
+  for (int off = 4 * lane; off < PB; off += 128) {
+    const int row = (int)v_swizzle(D, MODE, off) / rowB;
+    if (row >= ntok || !view.any(kBlock * col + row)) *reinterpret_cast<uint32_t *>(rec + PB + off) = 0u;
+  }
+  fence_proxy_async_smem();
 }
 
 // One FP16 page.
-template <int D, bool SLAB>
+template <int D, bool SLAB, bool ROWS>
 __device__ __forceinline__ void fp16_attend(uint8_t *rec, int ntok, int lane, const ScaleIdx &si,
                                             const uint32_t (&qf)[D / 16][2], float scale_log2,
-                                            SoftmaxState &st, float (&o)[D / 16][4]) {
+                                            SoftmaxState &st, float (&o)[D / 16][4], int col0, const RowView &view) {
   constexpr int PB = kBlock * D * 2;
   const int gid = lane >> 2, t4 = lane & 3;
-  if (ntok < kBlock) {
+  const int col[1] = {col0};
+  const bool part[1] = {ROWS && !view.whole_page(col0)};
+  if constexpr (ROWS) {
+    if (ntok < kBlock || part[0]) {
+      zero_unseen<D, AKV_MODE_FP16>(rec, ntok, col0, view, lane);
+      __syncwarp();
+    }
+  } else if (ntok < kBlock) {
     zero_tail<D, AKV_MODE_FP16>(rec, ntok, lane);
     __syncwarp();
   }
@@ -400,7 +467,7 @@ __device__ __forceinline__ void fp16_attend(uint8_t *rec, int ntok, int lane, co
   uint32_t b[1][2];
   const int nt[1] = {ntok};
   page_qk<D, AKV_MODE_FP16, SLAB>(rec, nullptr, none, gid, t4, qf, s[0]);
-  pages_softmax<D, 1>(s, nt, false, gid, scale_log2, st, o, b);
+  pages_softmax<D, 1, ROWS>(s, nt, false, gid, scale_log2, st, o, b, part, col, view);
   page_pv<D, AKV_MODE_FP16, SLAB>(rec + PB, nullptr, si, gid, t4, b[0][0], b[0][1], o);
 }
 
@@ -415,15 +482,24 @@ __device__ __forceinline__ void fp16_attend(uint8_t *rec, int ntok, int lane, co
 // but doubled the error tail of short sequences with outlier channels (66 of
 // 16.7 M outputs beyond 2e-3 of the reference's fp16 SDPA over the same pages,
 // against 0 without it).
-template <int D, int MODE, bool SLAB>
+template <int D, int MODE, bool SLAB, bool ROWS>
 __device__ __forceinline__ void slot_attend(uint8_t *rec, uint32_t rb, bool has2, int ntok0,
                                             int ntok1, int lane, int log2_group, const ScaleIdx &si,
                                             const uint32_t (&qf)[D / 16][2], float scale_log2,
-                                            SoftmaxState &st, float (&o)[D / 16][4]) {
+                                            SoftmaxState &st, float (&o)[D / 16][4], int col0, int col1,
+                                            const RowView &view) {
   constexpr int PB = kBlock * D * mode_bits(MODE) / 8;
   const int gid = lane >> 2, t4 = lane & 3;
   const int npages = has2 ? 2 : 1;
-  if (ntok0 < kBlock || (has2 && ntok1 < kBlock)) {
+  const int col[2] = {col0, col1};
+  const bool part[2] = {ROWS && !view.whole_page(col0), ROWS && has2 && !view.whole_page(col1)};
+  if constexpr (ROWS) {
+    if (ntok0 < kBlock || part[0] || (has2 && (ntok1 < kBlock || part[1]))) {
+      zero_unseen<D, MODE>(rec, ntok0, col0, view, lane);
+      if (has2) zero_unseen<D, MODE>(rec + rb, ntok1, col1, view, lane);
+      __syncwarp();
+    }
+  } else if (ntok0 < kBlock || (has2 && ntok1 < kBlock)) {
     if (ntok0 < kBlock) zero_tail<D, MODE>(rec, ntok0, lane);
     if (has2 && ntok1 < kBlock) zero_tail<D, MODE>(rec + rb, ntok1, lane);
     __syncwarp();
@@ -448,7 +524,7 @@ __device__ __forceinline__ void slot_attend(uint8_t *rec, uint32_t rb, bool has2
   }
   const int nt[2] = {ntok0, has2 ? ntok1 : 0};
   uint32_t b[2][2];
-  pages_softmax<D, 2>(s, nt, has2, gid, scale_log2, st, o, b);
+  pages_softmax<D, 2, ROWS>(s, nt, has2, gid, scale_log2, st, o, b, part, col, view);
   if constexpr (MODE == AKV_MODE_INT4) {
     page_pv<D, MODE, SLAB>(rec + PB, reinterpret_cast<const __half *>(rec + 2 * PB) + vgap, si, gid, t4,
                                  b[0][0], b[0][1], o);
@@ -467,7 +543,7 @@ __device__ __forceinline__ void slot_attend(uint8_t *rec, uint32_t rb, bool has2
 
 // Query words of this lane for item `item`: DK dims of query head (first head of
 // the item's group + gid), zeros for lanes past the group's head count.
-template <int D>
+template <int D, bool ROWS>
 __device__ __forceinline__ void load_query(const DecodeParams &p, int item, int gid, int t4,
                                            uint32_t (&qw)[D / 8]) {
   constexpr int DK = D / 4;
@@ -476,7 +552,13 @@ __device__ __forceinline__ void load_query(const DecodeParams &p, int item, int 
   const int kvh = r / p.qgroups, qg = r - kvh * p.qgroups;
   const int nq = min(8, p.gqa - 8 * qg);
   if (gid < nq) {
-    const __half *qp = p.q + (int64_t)b * p.q_bs + (int64_t)(kvh * p.gqa + 8 * qg + gid) * p.q_hs + t4 * DK;
+    const __half *qp = p.q + (int64_t)b * p.q_bs + t4 * DK;
+    if constexpr (ROWS) {  // row r of the KV head: query token r / heads_per_kv, head r % heads_per_kv
+      const int r = 8 * qg + gid, t = fdiv(r, p.fd_hpk);
+      qp += (int64_t)(kvh * p.heads_per_kv + (r - t * p.heads_per_kv)) * p.q_hs + (int64_t)t * p.q_ts;
+    } else {
+      qp += (int64_t)(kvh * p.gqa + 8 * qg + gid) * p.q_hs;
+    }
 #pragma unroll
     for (int i = 0; i < DK / 8; ++i) {
       const uint4 v = __ldg(reinterpret_cast<const uint4 *>(qp) + i);
@@ -499,9 +581,40 @@ __device__ __forceinline__ void query_fragments(const uint32_t (&qw)[D / 8], uin
   }
 }
 
+// The row positions of an item of a multi-row decode, and its query-head group.
+struct ItemRows {
+  int at_first, row0, n, at_lo, at_hi;  // position of query token 0; first row of the group, its rows
+};
+__device__ __forceinline__ ItemRows item_rows(const DecodeParams &p, int item) {
+  ItemRows v;
+  const int b = fdiv(item, p.fd_ipb);
+  const int held = kBlock * (p.seq_blocks ? max(0, min(__ldg(p.seq_blocks + b), p.columns)) : p.columns);
+  const int tokens = min(p.tokens ? __ldg(p.tokens + b) : p.uniform_tokens, held);
+  v.at_first = tokens - p.rows;
+  v.row0 = 8 * (item - fdiv(item, p.fd_qgroups) * p.qgroups);  // items are kv_heads * qgroups per sequence
+  v.n = min(8, p.gqa - v.row0);
+  v.at_lo = v.at_first + fdiv(v.row0, p.fd_hpk);
+  v.at_hi = v.at_first + fdiv(v.row0 + v.n - 1, p.fd_hpk);
+  return v;
+}
+__device__ __forceinline__ RowView row_view(const DecodeParams &p, int item, int t4) {
+  const ItemRows v = item_rows(p, item);
+  RowView r;
+  // Rows past the group's count repeat its last row: they only waste a lane.
+  r.at0 = v.at_first + fdiv(v.row0 + min(2 * t4, v.n - 1), p.fd_hpk);
+  r.at1 = v.at_first + fdiv(v.row0 + min(2 * t4 + 1, v.n - 1), p.fd_hpk);
+  r.at_lo = v.at_lo, r.at_hi = v.at_hi, r.window = p.window, r.sinks = p.sinks;
+  return r;
+}
+
 // SLAB: one scale per 16-token slab (group = 16 * head_dim), the
 // per-block-per-KV-head layout; false: per-row groups (32/64/128).
-template <int D, bool SLAB>
+// ROWS: a multi-row decode.  The "query heads" of a KV head are then its
+// rows x heads_per_kv (query token, query head) pairs, token-major, so 8 of them
+// share every page a warp streams; an item's entries are the page columns its
+// rows can see (the columns of the first `sinks` tokens, then those from the
+// oldest row's window on), and pages at the borders are masked by position.
+template <int D, bool SLAB, bool ROWS>
 __global__ void __launch_bounds__(DecodeTraits<D>::kMaxThreads, 1)
     decode_streamk_kernel(const DecodeParams p) {
   using T = DecodeTraits<D>;
@@ -537,6 +650,7 @@ __global__ void __launch_bounds__(DecodeTraits<D>::kMaxThreads, 1)
   uint32_t *slot_start = reinterpret_cast<uint32_t *>(ring + T::kRing + T::kSlots * 8);
   uint32_t *slot_meta = slot_start + T::kSlots;
   uint32_t *slot_phys = slot_meta + T::kSlots;
+  int2 *slot_cols = reinterpret_cast<int2 *>(slot_phys + T::kSlots);  // ROWS: the pages' columns
 
   const int lg = p.log2_group;
   ScaleIdx si;
@@ -571,8 +685,17 @@ __global__ void __launch_bounds__(DecodeTraits<D>::kMaxThreads, 1)
     nb = 0;
     if (e < e_end) {
       const int it = fdiv(e, p.fd_mb), bb = fdiv(it, p.fd_ipb);
-      nb = p.seq_blocks ? min(__ldg(p.seq_blocks + bb), mb) : mb;
-      raw = __ldg(p.table + (int64_t)bb * p.table_stride + (e - it * mb));
+      if constexpr (ROWS) {  // nb: the entry's column, raw a skip entry where the item sees nothing of it
+        const ItemRows v = item_rows(p, it);
+        const int first = max(p.lead, max(v.at_lo - p.window + 1, 0) / kBlock);
+        const int j = e - it * mb;
+        nb = j < p.lead ? j : first + (j - p.lead);
+        const int held = p.seq_blocks ? min(__ldg(p.seq_blocks + bb), p.columns) : p.columns;
+        if (nb < held && kBlock * nb <= v.at_hi) raw = __ldg(p.table + (int64_t)bb * p.table_stride + nb);
+      } else {
+        nb = p.seq_blocks ? min(__ldg(p.seq_blocks + bb), mb) : mb;
+        raw = __ldg(p.table + (int64_t)bb * p.table_stride + (e - it * mb));
+      }
     }
   };
   // Per lane (one page of the window each): the record's source offset, the
@@ -581,6 +704,7 @@ __global__ void __launch_bounds__(DecodeTraits<D>::kMaxThreads, 1)
   // lanes that lead a slot; a follower travels with its leader.
   int64_t w_src = 0, w_src2 = 0;
   uint32_t w_need = 0, w_meta = 0, w_mask = 0;
+  int w_col = 0, w_col2 = 0;  // ROWS: the lane's page column and its partner's
   auto prepare = [&](int w0, int64_t raw, int nb) {
     const int e = w0 + lane;
     bool ok = false, first = false;
@@ -589,7 +713,8 @@ __global__ void __launch_bounds__(DecodeTraits<D>::kMaxThreads, 1)
     if (e < e_end) {
       const int it = fdiv(e, p.fd_mb), j = e - it * mb;
       first = j == 0;
-      mode = j < nb ? desc_mode(raw) : AKV_MODE_SKIP;
+      mode = ROWS || j < nb ? desc_mode(raw) : AKV_MODE_SKIP;
+      if constexpr (ROWS) w_col = nb;
       rb = mode == AKV_MODE_FP16 ? rb16 : (mode == AKV_MODE_INT8 ? rb8 : rb4);
       const int64_t poff = desc_offset(raw);
       ok = mode != AKV_MODE_SKIP;
@@ -617,6 +742,7 @@ __global__ void __launch_bounds__(DecodeTraits<D>::kMaxThreads, 1)
     const uint32_t next = group & above;
     const int partner = grouped && !follower && next ? __ffs(next) - 1 : lane;
     w_src2 = __shfl_sync(0xffffffffu, w_src, partner);
+    if constexpr (ROWS) w_col2 = __shfl_sync(0xffffffffu, w_col, partner);
     const uint32_t pmeta = __shfl_sync(0xffffffffu, w_meta, partner);
     w_need = partner != lane ? 2u * rb : rb;
     if (partner != lane) w_meta |= 4u | (((pmeta >> 4) & 31u) << 9);
@@ -640,13 +766,15 @@ __global__ void __launch_bounds__(DecodeTraits<D>::kMaxThreads, 1)
   uint32_t qf[T::kTiles][2];
   {
     uint32_t qw[D / 8];
-    load_query<D>(p, first_item, gid, t4, qw);
+    load_query<D, ROWS>(p, first_item, gid, t4, qw);
     query_fragments<D>(qw, qf);
   }
   float o[T::kTiles][4];
 #pragma unroll
   for (int m = 0; m < T::kTiles; ++m) o[m][0] = o[m][1] = o[m][2] = o[m][3] = 0.f;
   SoftmaxState st{-INFINITY, -INFINITY, 0.f, 0.f};
+  RowView view{};
+  if constexpr (ROWS) view = row_view(p, first_item, t4);
   int cur_seg = 0;
 
   auto finalize = [&](int seg) {
@@ -684,8 +812,9 @@ __global__ void __launch_bounds__(DecodeTraits<D>::kMaxThreads, 1)
     st = SoftmaxState{-INFINITY, -INFINITY, 0.f, 0.f};
     if (cur_seg <= last_seg) {  // each warp meets only a few items: load the next query directly
       uint32_t qw[D / 8];
-      load_query<D>(p, first_item + cur_seg, gid, t4, qw);
+      load_query<D, ROWS>(p, first_item + cur_seg, gid, t4, qw);
       query_fragments<D>(qw, qf);
+      if constexpr (ROWS) view = row_view(p, first_item + cur_seg, t4);
     }
   };
 
@@ -721,6 +850,7 @@ __global__ void __launch_bounds__(DecodeTraits<D>::kMaxThreads, 1)
         slot_start[slot] = start;
         slot_phys[slot] = start_p;
         slot_meta[slot] = w_meta;
+        if constexpr (ROWS) slot_cols[slot] = make_int2(w_col, w_col2);
         // No proxy fence before the copy: every generic read of this ring
         // space has returned its value (consumed by the page math) already.
         const uint32_t bar = smem_u32(&bars[slot]);
@@ -752,15 +882,19 @@ __global__ void __launch_bounds__(DecodeTraits<D>::kMaxThreads, 1)
     }
     const int ntok = (int)((meta >> 4) & 31), ntok1 = (int)((meta >> 9) & 31);
     const bool has2 = (meta & 4u) != 0;
+    int2 cols = make_int2(0, 0);
+    if constexpr (ROWS) cols = slot_cols[slot];
     switch (meta & 3u) {
       case AKV_MODE_INT4:
-        slot_attend<D, AKV_MODE_INT4, SLAB>(rec, rb4, has2, ntok, ntok1, lane, lg, si, qf, p.scale_log2, st, o);
+        slot_attend<D, AKV_MODE_INT4, SLAB, ROWS>(rec, rb4, has2, ntok, ntok1, lane, lg, si, qf, p.scale_log2, st, o,
+                                                  cols.x, cols.y, view);
         break;
       case AKV_MODE_INT8:
-        slot_attend<D, AKV_MODE_INT8, SLAB>(rec, rb8, has2, ntok, ntok1, lane, lg, si, qf, p.scale_log2, st, o);
+        slot_attend<D, AKV_MODE_INT8, SLAB, ROWS>(rec, rb8, has2, ntok, ntok1, lane, lg, si, qf, p.scale_log2, st, o,
+                                                  cols.x, cols.y, view);
         break;
       default:
-        fp16_attend<D, SLAB>(rec, ntok, lane, si, qf, p.scale_log2, st, o);
+        fp16_attend<D, SLAB, ROWS>(rec, ntok, lane, si, qf, p.scale_log2, st, o, cols.x, view);
         break;
     }
     __syncwarp();
@@ -799,14 +933,26 @@ __device__ __forceinline__ bool merge_geom(const int32_t *header, MergeGeom &g) 
   return f[kMagic] == kHeaderMagic && f[kHeadDimF] == D;
 }
 
-// Write one merged row: the normalised fp16 output and/or the (acc, m, l) state.
+// Where the output rows lie.  heads_per_kv > 0: a multi-row decode, whose KV
+// head's row r is query token r / heads_per_kv of query head r % heads_per_kv.
+struct OutRows {
+  int64_t bs, hs, ts;
+  int32_t heads_per_kv;
+  // Element offset of row h = kvh * gqa + r of sequence b.
+  __device__ __forceinline__ int64_t at(int b, int h, int kvh, int r) const {
+    if (heads_per_kv == 0) return (int64_t)b * bs + (int64_t)h * hs;
+    const int t = r / heads_per_kv;
+    return (int64_t)b * bs + (int64_t)(kvh * heads_per_kv + (r - t * heads_per_kv)) * hs + (int64_t)t * ts;
+  }
+};
+
+// Write one merged row: the normalised fp16 output (at `out`) and/or the (acc, m, l) state.
 template <int D>
 __device__ __forceinline__ void store_row(int lane, int b, int h, int q_heads, float m, float l,
-                                          const float (&acc)[D / 32], __half *out, int64_t obs, int64_t ohs,
-                                          float *state) {
+                                          const float (&acc)[D / 32], __half *out, float *state) {
   constexpr int VEC = D / 32, RS = D + 2;
   if (out) {
-    __half *o = out + (int64_t)b * obs + (int64_t)h * ohs + VEC * lane;
+    __half *o = out + VEC * lane;
     const float inv = l > 0.f ? 1.f / l : 0.f;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) o[i] = __float2half_rn(acc[i] * inv);
@@ -827,9 +973,8 @@ __device__ __forceinline__ void store_row(int lane, int b, int h, int q_heads, f
 // Flattened work indices fit 31 bits (the plan checks), so int arithmetic.
 template <int D>
 __global__ void __launch_bounds__(128) merge_rows_kernel(const int32_t *__restrict__ header, int batch,
-                                                         int q_heads, __half *__restrict__ out, int64_t obs,
-                                                         int64_t ohs, float *__restrict__ state,
-                                                         int32_t *status) {
+                                                         int q_heads, __half *__restrict__ out, OutRows rows,
+                                                         float *__restrict__ state, int32_t *status) {
   constexpr int PS = D + 4, VEC = D / 32, CB = 8;
   grid_dependency_wait();  // the decode grid that wrote the workspace has completed
   allow_dependents_launch();
@@ -883,7 +1028,7 @@ __global__ void __launch_bounds__(128) merge_rows_kernel(const int32_t *__restri
       }
     }
   }
-  store_row<D>(lane, b, h, q_heads, m, l, acc, out, obs, ohs, state);
+  store_row<D>(lane, b, h, q_heads, m, l, acc, out ? out + rows.at(b, h, kvh, r) : nullptr, state);
 }
 
 // Fold contributors w, w + stride, ... (<= w_end) of `item`, query head n of its
@@ -972,7 +1117,7 @@ __device__ __forceinline__ void cta_fold(const FoldSmem<D> &sm, int warp, int la
 // and the 32 warp states fold in shared memory (cta_fold).
 template <int D>
 __global__ void __launch_bounds__(1024) merge_wide_kernel(const int32_t *__restrict__ header, int q_heads,
-                                                          __half *__restrict__ out, int64_t obs, int64_t ohs,
+                                                          __half *__restrict__ out, OutRows rows,
                                                           float *__restrict__ state, int32_t *status) {
   constexpr int VEC = D / 32, W = 32;
   __shared__ FoldSmem<D> sm;
@@ -1008,7 +1153,7 @@ __global__ void __launch_bounds__(1024) merge_wide_kernel(const int32_t *__restr
     for (int i = 1; i < VEC; ++i)
       if (lane == i) v = num[i];
     if (out)
-      out[(int64_t)b * obs + (int64_t)h * ohs + VEC * warp + lane] = __float2half_rn(v * (den > 0.f ? 1.f / den : 0.f));
+      out[rows.at(b, h, kvh, r) + VEC * warp + lane] = __float2half_rn(v * (den > 0.f ? 1.f / den : 0.f));
     if (state) {
       float *st = state + ((int64_t)b * q_heads + h) * (D + 2);
       st[VEC * warp + lane] = v;
@@ -1223,6 +1368,8 @@ struct Plan {
 // item) a warp gets at least, against its fixed cost (query load, copy
 // pipeline fill, partial write, one more merge contributor).
 constexpr int64_t kMinPagesPerWarp = 16;
+// Items one warp's range may touch: a slot's meta word holds the item in 16 bits.
+constexpr int kMaxSegments = 1 << 16;
 
 // CTAs of kMaxWarps warps the device holds at once (one per SM).  Constant per
 // device, so it is worked out (and the kernels' shared-memory limit raised)
@@ -1242,18 +1389,18 @@ static int device_ctas(int *out) {
     }
   }
   if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return AKV_ERR_CUDA;
-  int per_sm_slab = 0;
-  if (cudaFuncSetAttribute(decode_streamk_kernel<D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           T::kSmemMax) != cudaSuccess ||
-      cudaFuncSetAttribute(decode_streamk_kernel<D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           T::kSmemMax) != cudaSuccess)
+  // Every variant gets the same decomposition, so the least occupancy counts.
+  auto fit = [&](auto kernel) {
+    int n = 0;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmemMax) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, T::kMaxThreads, T::kSmemMax) != cudaSuccess)
+      return false;
+    per_sm = per_sm == 0 ? n : std::min(per_sm, n);
+    return true;
+  };
+  if (!fit(decode_streamk_kernel<D, false, false>) || !fit(decode_streamk_kernel<D, true, false>) ||
+      !fit(decode_streamk_kernel<D, false, true>) || !fit(decode_streamk_kernel<D, true, true>))
     return AKV_ERR_CUDA;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, decode_streamk_kernel<D, false>, T::kMaxThreads,
-                                                    T::kSmemMax) != cudaSuccess ||
-      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm_slab, decode_streamk_kernel<D, true>,
-                                                    T::kMaxThreads, T::kSmemMax) != cudaSuccess)
-    return AKV_ERR_CUDA;
-  per_sm = std::min(per_sm, per_sm_slab);  // both variants get the same decomposition
   if (per_sm < 1) return AKV_ERR_CUDA;
   *out = sms * per_sm;
   if (cacheable) cached[dev].store(sms * per_sm, std::memory_order_release);
@@ -1319,33 +1466,24 @@ extern "C" int64_t akv_workspace_bytes(int batch, int q_heads, int kv_heads, int
 }
 
 namespace akv {
-// Launch with programmatic stream serialization: the kernel may begin while its
-// predecessor in the stream finishes (it calls grid_dependency_wait() before
-// touching memory the predecessor may write or read).
-template <typename... Params, typename... Args>
-static cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem,
-                                    cudaStream_t s, Args... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
+// A multi-row decode's extra arguments; `q_heads` and `max_blocks` of the call are
+// then the rows per sequence (query heads x query tokens) and the page columns
+// an item may see.
+struct RowsArgs {
+  const int32_t *tokens;
+  int32_t uniform_tokens, rows, heads_per_kv, columns, window, sinks, lead;
+  int64_t q_ts;
+};
 
 // Validate, plan and launch the decode kernel.
 static int decode_launch(const void *arena, int64_t arena_bytes, const int64_t *table, int64_t table_stride,
                          const int32_t *seq_blocks, int32_t max_blocks, const void *query,
                          int64_t q_batch_stride, int64_t q_head_stride, int32_t batch, int32_t q_heads,
                          int32_t kv_heads, int32_t head_dim, int32_t group, float scale, int32_t splits,
-                         void *workspace, int64_t workspace_bytes, int32_t *dev_status, cudaStream_t s) {
+                         void *workspace, int64_t workspace_bytes, int32_t *dev_status, cudaStream_t s,
+                         const RowsArgs *rows = nullptr) {
   if (!arena || !table || !query || !workspace) return AKV_ERR_INVALID;
-  if (table_stride < max_blocks || arena_bytes < 0 || !isfinite(scale)) return AKV_ERR_INVALID;
+  if (table_stride < (rows ? rows->columns : max_blocks) || arena_bytes < 0 || !isfinite(scale)) return AKV_ERR_INVALID;
   if (((uintptr_t)arena & 15) || ((uintptr_t)query & 15) || ((uintptr_t)workspace & 15))
     return AKV_ERR_INVALID;
   if (q_batch_stride % 8 || q_head_stride % 8) return AKV_ERR_INVALID;
@@ -1359,7 +1497,8 @@ static int decode_launch(const void *arena, int64_t arena_bytes, const int64_t *
       make_plan(batch, q_heads, kv_heads, head_dim, max_blocks, splits, &pl, false) != AKV_OK)
     return AKV_ERR_INVALID;
   if (workspace_bytes < pl.bytes) return AKV_ERR_INVALID;
-  DecodeParams p;
+  if (rows && pl.smax > kMaxSegments) return AKV_ERR_UNSUPPORTED;
+  DecodeParams p = {};
   p.arena = (const uint8_t *)arena;
   p.arena_bytes = arena_bytes;
   p.table = table;
@@ -1387,14 +1526,24 @@ static int decode_launch(const void *arena, int64_t arena_bytes, const int64_t *
   p.header = (int32_t *)workspace;
   p.partials = (float *)((uint8_t *)workspace + kHeaderBytes);
   p.status = dev_status;
+  if (rows) {
+    p.tokens = rows->tokens, p.uniform_tokens = rows->uniform_tokens, p.rows = rows->rows;
+    p.heads_per_kv = rows->heads_per_kv, p.columns = rows->columns, p.window = rows->window;
+    p.sinks = rows->sinks, p.lead = rows->lead, p.q_ts = rows->q_ts;
+    p.fd_hpk = fast_div((uint32_t)rows->heads_per_kv);
+  }
   const bool slab = group == 16 * head_dim;
   cudaError_t err;
+  auto launch = [&](auto wide, auto kernel_slab_rows, auto kernel_rows, auto kernel_slab, auto kernel) {
+    return launch_dependent(rows ? (slab ? kernel_slab_rows : kernel_rows) : (slab ? kernel_slab : kernel), pl.ctas,
+                            pl.wpc * 32, pl.wpc * decltype(wide)::kWarpBytes, s, p);
+  };
   if (head_dim == 64)
-    err = launch_dependent(slab ? decode_streamk_kernel<64, true> : decode_streamk_kernel<64, false>, pl.ctas,
-                           pl.wpc * 32, pl.wpc * DecodeTraits<64>::kWarpBytes, s, p);
+    err = launch(DecodeTraits<64>{}, decode_streamk_kernel<64, true, true>, decode_streamk_kernel<64, false, true>,
+                 decode_streamk_kernel<64, true, false>, decode_streamk_kernel<64, false, false>);
   else
-    err = launch_dependent(slab ? decode_streamk_kernel<128, true> : decode_streamk_kernel<128, false>, pl.ctas,
-                           pl.wpc * 32, pl.wpc * DecodeTraits<128>::kWarpBytes, s, p);
+    err = launch(DecodeTraits<128>{}, decode_streamk_kernel<128, true, true>, decode_streamk_kernel<128, false, true>,
+                 decode_streamk_kernel<128, true, false>, decode_streamk_kernel<128, false, false>);
   return err == cudaSuccess ? AKV_OK : AKV_ERR_CUDA;
 }
 
@@ -1402,14 +1551,14 @@ static int decode_launch(const void *arena, int64_t arena_bytes, const int64_t *
 // (sequence, head) rows mean many contributors per row (a long sequence: one
 // CTA of 32 warps per row), many rows few contributors (one warp per row).
 template <int D>
-static cudaError_t merge_launch(const int32_t *header, int batch, int q_heads, __half *out, int64_t obs,
-                                int64_t ohs, float *state, int32_t *status, cudaStream_t s) {
+static cudaError_t merge_launch(const int32_t *header, int batch, int q_heads, __half *out, OutRows to,
+                                float *state, int32_t *status, cudaStream_t s) {
   const int rows = batch * q_heads;
   if (rows < 2 * 148)
-    return launch_dependent(merge_wide_kernel<D>, dim3(q_heads, batch), 1024, 0, s, header, q_heads, out, obs,
-                            ohs, state, status);
-  return launch_dependent(merge_rows_kernel<D>, dim3((rows + 3) / 4), 128, 0, s, header, batch, q_heads, out,
-                          obs, ohs, state, status);
+    return launch_dependent(merge_wide_kernel<D>, dim3(q_heads, batch), 1024, 0, s, header, q_heads, out, to, state,
+                            status);
+  return launch_dependent(merge_rows_kernel<D>, dim3((rows + 3) / 4), 128, 0, s, header, batch, q_heads, out, to,
+                          state, status);
 }
 }  // namespace akv
 
@@ -1434,11 +1583,10 @@ extern "C" int akv_merge(const void *workspace, int32_t batch, int32_t q_heads, 
   if (head_dim != 64 && head_dim != 128) return AKV_ERR_UNSUPPORTED;
   const int32_t *header = (const int32_t *)workspace;
   cudaStream_t s = (cudaStream_t)stream;
+  const OutRows to{out_batch_stride, out_head_stride, 0, 0};
   const cudaError_t err =
-      head_dim == 64 ? merge_launch<64>(header, batch, q_heads, (__half *)out, out_batch_stride, out_head_stride,
-                                        state_out, dev_status, s)
-                     : merge_launch<128>(header, batch, q_heads, (__half *)out, out_batch_stride,
-                                         out_head_stride, state_out, dev_status, s);
+      head_dim == 64 ? merge_launch<64>(header, batch, q_heads, (__half *)out, to, state_out, dev_status, s)
+                     : merge_launch<128>(header, batch, q_heads, (__half *)out, to, state_out, dev_status, s);
   return err == cudaSuccess ? AKV_OK : AKV_ERR_CUDA;
 }
 
@@ -1540,6 +1688,90 @@ extern "C" int akv_packed_attention(const void *arena, int64_t arena_bytes, cons
   if (st != AKV_OK) return st;
   return akv_merge(workspace, batch, q_heads, head_dim, out, out_batch_stride, out_head_stride,
                    nullptr, dev_status, stream);
+}
+
+// ================================================ multi-row decode (chunks)
+namespace akv {
+// Positions stay in 32 bits with room for position - window: tokens and window
+// are at most 2^30.
+constexpr int32_t kMaxTokens = 1 << 30;
+
+// Page columns an item (8 rows of a KV head) of a multi-row decode may see: the
+// columns of the first `sinks` tokens (`lead`), then those of the tokens from the
+// oldest row's window to the newest row (at most window + span - 1 tokens,
+// starting anywhere in a page).  Without a window: every column.
+static int visible_columns(int max_blocks, int rows, int heads_per_kv, int window, int sinks, int *lead) {
+  if (window <= 0) {
+    *lead = 0;
+    return max_blocks;
+  }
+  *lead = (int)std::min<int64_t>(max_blocks, ((int64_t)sinks + kBlock - 1) / kBlock);
+  const int span = std::min(rows, 7 / heads_per_kv + 2);
+  const int64_t near = ((int64_t)window + span - 1 + kBlock - 2) / kBlock + 1;
+  return *lead + (int)std::min<int64_t>(max_blocks - *lead, near);
+}
+
+struct ChunkPlan {
+  int rows_total;  // rows of all KV heads of a sequence
+  int columns;     // page columns an item may see
+  RowsArgs rows;
+};
+static int chunk_plan(int batch, int rows, int q_heads, int kv_heads, int head_dim, int max_blocks, int window,
+                      int sinks, ChunkPlan *out) {
+  if (batch <= 0 || batch > 65535 || rows <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || max_blocks < 0)
+    return AKV_ERR_INVALID;
+  if (sinks < 0 || (window <= 0 && sinks > 0)) return AKV_ERR_INVALID;
+  if (head_dim != 64 && head_dim != 128) return AKV_ERR_UNSUPPORTED;
+  const int64_t total = (int64_t)q_heads * rows;
+  if (max_blocks > kMaxTokens / kBlock || rows > kMaxTokens || total * batch >= (1ll << 31)) return AKV_ERR_UNSUPPORTED;
+  out->rows_total = (int)total;
+  RowsArgs &r = out->rows;
+  r = {};
+  r.rows = rows;
+  r.heads_per_kv = q_heads / kv_heads;
+  out->columns = visible_columns(max_blocks, rows, r.heads_per_kv, window, sinks, &r.lead);
+  r.columns = max_blocks;
+  r.window = window <= 0 ? kMaxTokens : std::min(window, kMaxTokens);
+  r.sinks = sinks;
+  return AKV_OK;
+}
+}  // namespace akv
+
+extern "C" int64_t akv_chunk_workspace_bytes(int32_t batch, int32_t rows, int32_t q_heads, int32_t kv_heads,
+                                             int32_t head_dim, int32_t max_blocks, int32_t window, int32_t sinks,
+                                             int32_t splits) {
+  ChunkPlan c;
+  Plan pl;
+  if (chunk_plan(batch, rows, q_heads, kv_heads, head_dim, max_blocks, window, sinks, &c) != AKV_OK) return -1;
+  if (make_plan(batch, c.rows_total, kv_heads, head_dim, c.columns, splits, &pl) != AKV_OK) return -1;
+  return pl.smax > kMaxSegments ? -1 : pl.bytes;
+}
+
+extern "C" int akv_chunk_attention(const void *arena, int64_t arena_bytes, const int64_t *table, int64_t table_stride,
+                                   const int32_t *seq_blocks, int32_t max_blocks, const int32_t *tokens,
+                                   int32_t uniform_tokens, const void *query, int64_t q_batch_stride,
+                                   int64_t q_head_stride, int64_t q_token_stride, int32_t batch, int32_t rows,
+                                   int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t group, float scale,
+                                   int32_t window, int32_t sinks, int32_t splits, void *out, int64_t out_batch_stride,
+                                   int64_t out_head_stride, int64_t out_token_stride, void *workspace,
+                                   int64_t workspace_bytes, int32_t *dev_status, void *stream) {
+  if (!out || q_token_stride % 8 || (!tokens && uniform_tokens < 0)) return AKV_ERR_INVALID;
+  ChunkPlan c;
+  if (int st = chunk_plan(batch, rows, q_heads, kv_heads, head_dim, max_blocks, window, sinks, &c)) return st;
+  c.rows.tokens = tokens;
+  c.rows.uniform_tokens = std::min(uniform_tokens, kMaxTokens);
+  c.rows.q_ts = q_token_stride;
+  cudaStream_t s = (cudaStream_t)stream;
+  if (int st = decode_launch(arena, arena_bytes, table, table_stride, seq_blocks, c.columns, query, q_batch_stride,
+                             q_head_stride, batch, c.rows_total, kv_heads, head_dim, group, scale, splits, workspace,
+                             workspace_bytes, dev_status, s, &c.rows))
+    return st;
+  const OutRows to{out_batch_stride, out_head_stride, out_token_stride, c.rows.heads_per_kv};
+  const int32_t *header = (const int32_t *)workspace;
+  const cudaError_t err =
+      head_dim == 64 ? merge_launch<64>(header, batch, c.rows_total, (__half *)out, to, nullptr, dev_status, s)
+                     : merge_launch<128>(header, batch, c.rows_total, (__half *)out, to, nullptr, dev_status, s);
+  return err == cudaSuccess ? AKV_OK : AKV_ERR_CUDA;
 }
 
 // ===================================================== allocation-free variant

@@ -56,6 +56,7 @@ extern "C" {
  * may leave only one of them, but the word is nonzero after any error. */
 #define AKV_DEV_BAD_DESCRIPTOR 1 /* descriptor outside the arena or misaligned; page skipped */
 #define AKV_DEV_TIMEOUT 2        /* a bounded wait on a bulk copy gave up */
+#define AKV_DEV_BAD_PARENT 4     /* akv_fork_pages: a parent outside the batch; its child's row is empty */
 
 /* Page modes (descriptor bits 0-1). */
 #define AKV_MODE_SKIP 0
@@ -260,6 +261,76 @@ int akv_packed_attention(const void *arena, int64_t arena_bytes, const int64_t *
                          int32_t group, float scale, int32_t splits, void *out,
                          int64_t out_batch_stride, int64_t out_head_stride, void *workspace,
                          int64_t workspace_bytes, int32_t *dev_status, void *stream);
+
+/* Causal attention of the last `rows` tokens of every sequence over its pages
+ * (a prompt's next chunk, or drafted tokens to verify), optionally through a
+ * sliding window with visible first tokens.  rows = 1 is the single-token
+ * decode with a window.
+ *   tokens: int32 [batch], tokens each sequence holds, this call's rows
+ *     included (NULL: uniform_tokens each); a count beyond the pages of the
+ *     sequence is taken as what its pages hold.  Page column j holds positions
+ *     16j .. 16j + 15; a skip entry (or a row past a page's valid count) is
+ *     never attended.
+ *   query: fp16 [batch][q_heads][rows][head_dim] with the given strides; row i
+ *     stands at position tokens - rows + i and sees the positions up to its own.
+ *     A row at a negative position (a sequence shorter than `rows`) and a row
+ *     that sees no resident token get zeros.
+ *   window: > 0: a row sees its last `window` positions, its own included, and
+ *     the sequence's first `sinks` positions; <= 0: every position (sinks 0).
+ * Only the pages that some row sees are read.  V values of tokens that no row
+ * sees never reach the output, whatever they hold; a non-finite V value of a
+ * token that some row sees may reach the other rows of the call.
+ * workspace: akv_chunk_workspace_bytes bytes, 16-byte aligned, with the rules of
+ * akv_workspace_bytes.  No counterpart in the reference, whose packed kernel
+ * takes one query token and no window (triton_decode.py:87). */
+int akv_chunk_attention(const void *arena, int64_t arena_bytes, const int64_t *table,
+                        int64_t table_stride, const int32_t *seq_blocks, int32_t max_blocks,
+                        const int32_t *tokens, int32_t uniform_tokens, const void *query,
+                        int64_t q_batch_stride, int64_t q_head_stride, int64_t q_token_stride,
+                        int32_t batch, int32_t rows, int32_t q_heads, int32_t kv_heads,
+                        int32_t head_dim, int32_t group, float scale, int32_t window, int32_t sinks,
+                        int32_t splits, void *out, int64_t out_batch_stride,
+                        int64_t out_head_stride, int64_t out_token_stride, void *workspace,
+                        int64_t workspace_bytes, int32_t *dev_status, void *stream);
+
+/* Bytes of akv_chunk_attention's workspace on the current device (-1 for
+ * invalid or unsupported arguments). */
+int64_t akv_chunk_workspace_bytes(int32_t batch, int32_t rows, int32_t q_heads, int32_t kv_heads,
+                                  int32_t head_dim, int32_t max_blocks, int32_t window,
+                                  int32_t sinks, int32_t splits);
+
+/* Page tables of `children` new sequences that continue given parents, for
+ * `layers` layers at once: child i's row is its parent's row of
+ * table[layer][batch][columns] (strides in entries), parents[i] in [0, batch).
+ * The child shares the parent's pages, except the half-filled page that its next
+ * token goes to (column tokens / 16 when tokens is not a multiple of 16; tokens
+ * per parent, NULL: uniform_tokens): where fresh[layer][child] is a descriptor
+ * (not 0) of a free slot of that page's precision, the page is copied there and
+ * the child's entry names the copy.  fresh may be NULL (share everything).
+ * out_table: [layers][children][columns], contiguous, apart from `table`.  Fresh
+ * slots must be distinct and named by no table.  No counterpart in the
+ * reference, whose cache holds one sequence (packed_decode.py:108-133). */
+int akv_fork_pages(const int64_t *table, int64_t layer_stride, int64_t seq_stride, int32_t layers,
+                   int32_t batch, int32_t columns, const int32_t *tokens, int32_t uniform_tokens,
+                   const int64_t *parents, int32_t children, const int64_t *fresh,
+                   int64_t *out_table, void *arena, int64_t arena_bytes, int heads, int head_dim,
+                   int group, int32_t *dev_status, void *stream);
+
+/* Copy the pages that table[entries] names into another arena and write the
+ * entries that name the copies to out_table: each page moves once, however many
+ * entries share it, to the next slot of its precision in the order in which the
+ * table first names it.  slots: host int64[6], first byte and slot count of the
+ * target's INT4, INT8 and FP16 slots (record-sized steps).  Pages past a slot count
+ * set AKV_DEV_BAD_DESCRIPTOR and their entries become skip entries.  The source
+ * arena and table are left as they are; arenas and tables must not overlap.
+ * workspace: akv_compact_workspace_bytes bytes, 16-byte aligned.  No counterpart
+ * in the reference, which allocates every page by itself (packed_decode.py:144). */
+int akv_compact_pages(const int64_t *table, int64_t entries, int64_t *out_table, const void *arena,
+                      int64_t arena_bytes, void *into, int64_t into_bytes, const int64_t *slots,
+                      int heads, int head_dim, int group, void *workspace, int64_t workspace_bytes,
+                      int32_t *dev_status, void *stream);
+int64_t akv_compact_workspace_bytes(int64_t entries, int64_t arena_bytes, int heads, int head_dim,
+                                    int group);
 
 /* Allocation-free akv_packed_attention.  No counterpart in the reference: it
  * exists for callers that cannot allocate device memory -- hosts that reserve
