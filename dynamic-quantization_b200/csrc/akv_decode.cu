@@ -47,6 +47,7 @@
 #include <atomic>
 #include <mutex>
 
+#include "akv_chunk.cuh"
 #include "akv_common.cuh"
 
 namespace akv {
@@ -1711,6 +1712,9 @@ static int visible_columns(int max_blocks, int rows, int heads_per_kv, int windo
   return *lead + (int)std::min<int64_t>(max_blocks - *lead, near);
 }
 
+// Whether a chunk of `rows_kv` rows per KV head runs on the tcgen05 tiles.
+static bool use_tiles(int64_t rows_kv) { return rows_kv > 8; }
+
 struct ChunkPlan {
   int rows_total;  // rows of all KV heads of a sequence
   int columns;     // page columns an item may see
@@ -1743,6 +1747,7 @@ extern "C" int64_t akv_chunk_workspace_bytes(int32_t batch, int32_t rows, int32_
   ChunkPlan c;
   Plan pl;
   if (chunk_plan(batch, rows, q_heads, kv_heads, head_dim, max_blocks, window, sinks, &c) != AKV_OK) return -1;
+  if (use_tiles(rows * c.rows.heads_per_kv)) return kHeaderBytes;
   if (make_plan(batch, c.rows_total, kv_heads, head_dim, c.columns, splits, &pl) != AKV_OK) return -1;
   return pl.smax > kMaxSegments ? -1 : pl.bytes;
 }
@@ -1762,6 +1767,21 @@ extern "C" int akv_chunk_attention(const void *arena, int64_t arena_bytes, const
   c.rows.uniform_tokens = std::min(uniform_tokens, kMaxTokens);
   c.rows.q_ts = q_token_stride;
   cudaStream_t s = (cudaStream_t)stream;
+  if (use_tiles(rows * c.rows.heads_per_kv)) {
+    if (!arena || !table || !query || table_stride < max_blocks || arena_bytes < 0 || !isfinite(scale)) return AKV_ERR_INVALID;
+    if (((uintptr_t)arena & 15) || ((uintptr_t)query & 15) || q_batch_stride % 8 || q_head_stride % 8) return AKV_ERR_INVALID;
+    const int lg = ilog2_exact(group);
+    if (lg < 0 || (group != 32 && group != 64 && group != 128 && group != 16 * head_dim)) return AKV_ERR_UNSUPPORTED;
+    ChunkArgs a = {};
+    a.arena = (const uint8_t *)arena, a.arena_bytes = arena_bytes, a.table = table, a.table_stride = table_stride;
+    a.seq_blocks = seq_blocks, a.columns = max_blocks, a.tokens = tokens, a.uniform_tokens = c.rows.uniform_tokens;
+    a.q = (const __half *)query, a.q_bs = q_batch_stride, a.q_hs = q_head_stride, a.q_ts = q_token_stride;
+    a.out = (__half *)out, a.o_bs = out_batch_stride, a.o_hs = out_head_stride, a.o_ts = out_token_stride;
+    a.batch = batch, a.rows = rows, a.q_heads = q_heads, a.kv_heads = kv_heads, a.head_dim = head_dim;
+    a.log2_group = lg, a.window = c.rows.window, a.sinks = c.rows.sinks, a.lead = c.rows.lead;
+    a.scale = scale, a.status = dev_status, a.stream = s;
+    return chunk_tiles_launch(a);
+  }
   if (int st = decode_launch(arena, arena_bytes, table, table_stride, seq_blocks, c.columns, query, q_batch_stride,
                              q_head_stride, batch, c.rows_total, kv_heads, head_dim, group, scale, splits, workspace,
                              workspace_bytes, dev_status, s, &c.rows))
