@@ -18,6 +18,7 @@
 // fp16(int * float(scale)), once per CTA and tile.  Waits are bounded: a role whose
 // wait runs out reports AKV_DEV_TIMEOUT and leaves its loop.
 #include <math.h>
+#include <stddef.h>
 
 #include <algorithm>
 #include <atomic>
@@ -82,6 +83,24 @@ __device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t *r) {
       "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(addr)
       : "memory");
 }
+// Shared memory by 32-bit address.
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ void lds64(uint32_t a, uint32_t (&v)[2]) {
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void lds128(uint32_t a, uint32_t (&v)[4]) {
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+               : "r"(a)
+               : "memory");
+}
+__device__ __forceinline__ void sts128(uint32_t a, const uint32_t (&v)[4]) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+}
 template <int N>
 __device__ __forceinline__ void set_registers_up() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -113,26 +132,22 @@ constexpr uint32_t mma_idesc(int n, bool b_mn_major) {
 
 constexpr int kTilePages = 8;
 constexpr int kTileTokens = kTilePages * kBlock;
-constexpr int kSlots = 4;       // operand tiles: K0 V0 K1 V1 ...
+constexpr int kMaxSlots = 8;    // operand tiles: K0 V0 K1 V1 ...
 constexpr int kItems = 8;       // half tiles of raw records in flight
 constexpr int kMetas = 8;       // the loader runs at most 5 tiles ahead of the softmax
 constexpr int kRawRing = 32768;
 constexpr int kTmemCols = 512;
-constexpr int kThreads = 512;
-// Registers a thread: at launch, and after the split (softmax, dequantisation, loader and MMA warpgroups).
-constexpr int kLaunchRegs = 128, kSoftmaxRegs = 192, kDequantRegs = 80, kIssueRegs = 48;
-static_assert(2 * kSoftmaxRegs + kDequantRegs + kIssueRegs <= 4 * kLaunchRegs, "a warpgroup would wait for registers");
 constexpr uint32_t kTmemS = 0, kTmemO = 256;  // S/P of row tile x at 128 x, O at 256 + 128 x
 
-struct TileMeta {
+struct __align__(16) TileMeta {
   int32_t col[kTilePages];
   uint32_t page[kTilePages];  // mode | valid tokens << 2; 0: no page
-  int64_t src[kTilePages];    // byte offset of the KV head's record
-  uint32_t last, whole;       // no tile follows; every row of the CTA sees every token
+  int64_t src[kTilePages];    // byte offset of the KV head's record (page kernel)
+  uint32_t last, whole, none;  // no tile follows; every row of the CTA sees every token; there is no tile at all
 };
 
 struct ChunkBars {
-  uint64_t raw_full[kItems], raw_empty[kItems], kv_full[kSlots], kv_empty[kSlots], q_full, s_full[2], p_full[2],
+  uint64_t raw_full[kItems], raw_empty[kItems], kv_full[kMaxSlots], kv_empty[kMaxSlots], q_full, s_full[2], p_full[2],
       o_full[2];
 };
 
@@ -143,10 +158,8 @@ struct ChunkShared {
   uint32_t tmem;
 };
 
-template <int D, int NT>
-constexpr int chunk_smem_bytes() {
-  return (NT + kSlots) * 128 * D * 2 + kRawRing + (int)sizeof(ChunkShared);
-}
+
+static_assert(offsetof(ChunkShared, meta) % 16 == 0 && sizeof(TileMeta) % 16 == 0, "lists move 16 bytes at a time");
 
 struct ChunkParams {
   ChunkArgs a;
@@ -261,7 +274,7 @@ __device__ __forceinline__ void chunk_load(const ChunkParams &p, ChunkShared &sh
     bool whole = true;
     if (lane < kTilePages) whole = (m.page[lane] >> 2) == kBlock && view.whole_page(m.col[lane]);
     whole = __all_sync(0xffffffffu, whole);
-    if (lane == 0) m.last = last, m.whole = whole;
+    if (lane == 0) m.last = last, m.whole = whole, m.none = 0;
     __syncwarp();
     for (int part = 0; part < 4; ++part) {  // K of pages 0-3, of 4-7, then V
       const int kv = part >> 1, i = 4 * (part & 1) + (lane & 3);
@@ -332,31 +345,37 @@ __device__ __forceinline__ void dequant_page(const uint8_t *raw, const __half *s
                                              int token0, int lane, bool check, Seen seen) {
   constexpr int NC = D / 16;
   constexpr int BYTES = MODE == AKV_MODE_FP16 ? 16 : (MODE == AKV_MODE_INT8 ? 8 : 4);  // of 8 elements
+  // Chunk c holds elements 256 c + 8 lane + [0, 8): row kRows c + row0, unit `unit`.
+  // Both swizzles are XORs of bits that c alone (or c and the lane apart) sets, so
+  // an address is a lane constant, one XOR with a constant and an immediate.
+  constexpr int kUnits = D / 8, kRows = 32 / kUnits;
+  const int row0 = lane / kUnits, unit = lane % kUnits;
+  const uint32_t dst0 = smem_u32(tile) + (uint32_t)((unit >> 3) * kPanel + (token0 + row0) * 128 + (((unit & 7) ^ row0) << 4));
+  const uint32_t src0 = smem_u32(raw);
+  const __half *sc = SLAB ? scales : scales + ((8 * lane) >> log2_group);
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    const int e = 256 * c + 8 * lane, row = e / D, unit = (e % D) / 8;
-    const int o = e / 8 * BYTES;
-    const uint8_t *src = raw + (VPAY ? (int)v_swizzle(D, MODE, o) : o);
+    const uint32_t src = src0 + (uint32_t)((BYTES * lane) ^ (VPAY ? v_chunk_xor<D>(MODE, c, lane) : 0)) + 32 * BYTES * c;
     uint32_t h[4];
     if constexpr (MODE == AKV_MODE_FP16) {
-      const uint4 w = *reinterpret_cast<const uint4 *>(src);
-      h[0] = w.x, h[1] = w.y, h[2] = w.z, h[3] = w.w;
+      lds128(src, h);
     } else {
-      const uint32_t s1 = __half_as_ushort(scales[SLAB ? 0 : e >> log2_group]), s = s1 | (s1 << 16);
+      const uint32_t s1 = __half_as_ushort(sc[SLAB ? 0 : (256 * c) >> log2_group]), s = s1 | (s1 << 16);
       if constexpr (MODE == AKV_MODE_INT8) {
-        const uint2 w = *reinterpret_cast<const uint2 *>(src);
-        h[0] = hmul2(int8_to_f16x2(prmt(w.x, 0, 0x1100)), s), h[1] = hmul2(int8_to_f16x2(prmt(w.x, 0, 0x3322)), s);
-        h[2] = hmul2(int8_to_f16x2(prmt(w.y, 0, 0x1100)), s), h[3] = hmul2(int8_to_f16x2(prmt(w.y, 0, 0x3322)), s);
+        uint32_t w[2];
+        lds64(src, w);
+        h[0] = hmul2(int8_to_f16x2(prmt(w[0], 0, 0x1100)), s), h[1] = hmul2(int8_to_f16x2(prmt(w[0], 0, 0x3322)), s);
+        h[2] = hmul2(int8_to_f16x2(prmt(w[1], 0, 0x1100)), s), h[3] = hmul2(int8_to_f16x2(prmt(w[1], 0, 0x3322)), s);
       } else {
-        const uint32_t w = *reinterpret_cast<const uint32_t *>(src);
+        const uint32_t w = lds32(src);
         const uint32_t e04 = hmul2(int4_lo_to_f16x2(w), s), e15 = hmul2(int4_hi_to_f16x2(w), s);
         const uint32_t e26 = hmul2(int4_lo_to_f16x2(w >> 8), s), e37 = hmul2(int4_hi_to_f16x2(w >> 8), s);
         h[0] = prmt(e04, e15, 0x5410), h[1] = prmt(e26, e37, 0x5410);
         h[2] = prmt(e04, e15, 0x7632), h[3] = prmt(e26, e37, 0x7632);
       }
     }
-    if (VPAY && check && !seen(row)) h[0] = h[1] = h[2] = h[3] = 0u;
-    *reinterpret_cast<uint4 *>(tile + panel_offset(token0 + row, unit)) = make_uint4(h[0], h[1], h[2], h[3]);
+    if (VPAY && check && !seen(kRows * c + row0)) h[0] = h[1] = h[2] = h[3] = 0u;
+    sts128((dst0 ^ (((kRows * c) & 7) << 4)) + kRows * 128 * c, h);
   }
 }
 
@@ -364,6 +383,7 @@ template <int D, bool SLAB>
 __device__ __forceinline__ void chunk_dequant(const ChunkParams &p, ChunkShared &sh, const uint8_t *ring, uint8_t *tiles,
                                               const ChunkView &view, int warp, int lane) {
   constexpr int kOperand = 128 * D * 2;
+  constexpr int kSlots = 4;
   const int lg = p.a.log2_group;
   bool dead = false;
   for (int n = 0; !dead; ++n) {
@@ -421,7 +441,7 @@ __device__ __forceinline__ void chunk_dequant(const ChunkParams &p, ChunkShared 
 // ---------------------------------------------------------------- MMA issue
 // One thread issues every MMA; they execute in the order of issue, so a row
 // tile's S may overwrite the P that the MMA before it read.
-template <int D, int NT>
+template <int D, int NT, int kSlots>
 __device__ __forceinline__ void chunk_mma(const ChunkParams &p, ChunkShared &sh, const uint8_t *q_tiles,
                                           const uint8_t *tiles, uint32_t tmem) {
   constexpr int kOperand = 128 * D * 2;
@@ -444,6 +464,10 @@ __device__ __forceinline__ void chunk_mma(const ChunkParams &p, ChunkShared &sh,
                 operand_desc(kv0 + slot * kOperand + k * 2048, kPanel, 1024), kPv, accumulate || k > 0);
   };
   bool ok = wait(bar.q_full, 0) && wait(bar.kv_full[0], 0);
+  if (ok && sh.meta[0].none) {  // nothing to attend: the softmax only has to know
+    for (int x = 0; x < NT; ++x) mbar_arrive(smem_u32(&bar.s_full[x]));
+    return;
+  }
   if (ok) {
     tc_fence_after();
 #pragma unroll
@@ -526,6 +550,7 @@ __device__ __forceinline__ void chunk_softmax(const ChunkParams &p, ChunkShared 
     tc_fence_after();
     const TileMeta &meta = sh.meta[j % kMetas];
     const bool last = meta.last;
+    if (meta.none) break;
     float s[128];
 #pragma unroll
     for (int i = 0; i < 4; ++i) tc_ld32(ts + 32 * i, s + 32 * i);
@@ -541,10 +566,13 @@ __device__ __forceinline__ void chunk_softmax(const ChunkParams &p, ChunkShared 
           if (!((bits >> i) & 1u)) s[kBlock * g + i] = kNegInf;
       }
     }
-    float top = s[0];
+    float tops[8];
 #pragma unroll
-    for (int i = 1; i < 128; ++i) top = fmaxf(top, s[i]);
-    top *= c;
+    for (int i = 0; i < 8; ++i) tops[i] = s[i];
+#pragma unroll
+    for (int i = 8; i < 128; ++i) tops[i % 8] = fmaxf(tops[i % 8], s[i]);
+    const float top = c * fmaxf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])),
+                                fmaxf(fmaxf(tops[4], tops[5]), fmaxf(tops[6], tops[7])));
     // S of this tile came after O of the tile before it, so O is at rest here.
     if (__any_sync(0xffffffffu, top > m + kSlack)) {
       const float n = fmaxf(m, top);
@@ -582,7 +610,8 @@ __device__ __forceinline__ void chunk_softmax(const ChunkParams &p, ChunkShared 
     if (lane == 0) mbar_arrive(smem_u32(&sh.bars.p_full[x]));
     if (last) break;
   }
-  if (!dead && !mbar_wait_bounded(smem_u32(&sh.bars.o_full[x]), 0)) dead = true;
+  const bool none = sh.meta[0].none;  // set once, for a CTA without a tile
+  if (!dead && !none && !mbar_wait_bounded(smem_u32(&sh.bars.o_full[x]), 0)) dead = true;
   if (dead) {
     if (lane == 0) set_status(p.a.status, AKV_DEV_TIMEOUT);
     return;
@@ -615,32 +644,63 @@ __device__ __forceinline__ void chunk_softmax(const ChunkParams &p, ChunkShared 
   }
 }
 
-template <int D, bool SLAB, int NT>
-__global__ void __launch_bounds__(kThreads, 1) chunk_tiles_kernel(const __grid_constant__ ChunkParams p) {
-  constexpr int kOperand = 128 * D * 2;
-  extern __shared__ __align__(1024) uint8_t smem[];
-  uint8_t *q_tiles = smem, *tiles = smem + NT * kOperand, *ring = tiles + kSlots * kOperand;
-  ChunkShared &sh = *reinterpret_cast<ChunkShared *>(ring + kRawRing);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+// ---------------------------------------------------------- CTA set-up
+__device__ __forceinline__ void chunk_begin(ChunkShared &sh, int nt, int kv_arrivals, int alloc_warp) {
   if (threadIdx.x == 0) {
     ChunkBars &bar = sh.bars;
     for (int i = 0; i < kItems; ++i) mbar_init(smem_u32(&bar.raw_full[i]), 1), mbar_init(smem_u32(&bar.raw_empty[i]), 4);
-    for (int i = 0; i < kSlots; ++i) mbar_init(smem_u32(&bar.kv_full[i]), 4), mbar_init(smem_u32(&bar.kv_empty[i]), 1);
-    mbar_init(smem_u32(&bar.q_full), 4 * NT);
+    for (int i = 0; i < kMaxSlots; ++i)
+      mbar_init(smem_u32(&bar.kv_full[i]), kv_arrivals), mbar_init(smem_u32(&bar.kv_empty[i]), 1);
+    mbar_init(smem_u32(&bar.q_full), 4 * nt);
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&bar.s_full[i]), 1);
       mbar_init(smem_u32(&bar.p_full[i]), 4);
       mbar_init(smem_u32(&bar.o_full[i]), 1);
     }
     fence_mbar_init();
+    sh.meta[0].none = 0;
   }
-  if (warp == 13) {
+  if ((int)(threadIdx.x >> 5) == alloc_warp) {
     tmem_alloc(smem_u32(&sh.tmem), kTmemCols);
     tmem_release_permit();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+}
+__device__ __forceinline__ void chunk_end(uint32_t tmem, int alloc_warp) {
+  tc_fence_before();
+  __syncthreads();
+  if ((int)(threadIdx.x >> 5) == alloc_warp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+template <int D>
+__device__ __forceinline__ void chunk_rows_role(const ChunkParams &p, ChunkShared &sh, const ChunkView &view, int b,
+                                                int kvh, int x, int w, int lane, uint8_t *q_tile, uint32_t tmem) {
+  load_rows<D>(p, view, b, kvh, x, w, lane, q_tile);
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) mbar_arrive(smem_u32(&sh.bars.q_full));
+  chunk_softmax<D>(p, sh, view, b, kvh, x, w, lane, tmem);
+}
+
+// ============================================== pages dequantised in the kernel
+constexpr int kPageSlots = 4;
+// Registers a thread: at launch, and after the split (softmax, dequantisation, loader and MMA warpgroups).
+constexpr int kPageThreads = 512;
+constexpr int kPageRegs = 128, kSoftmaxRegs = 192, kDequantRegs = 80, kIssueRegs = 48;
+static_assert(2 * kSoftmaxRegs + kDequantRegs + kIssueRegs <= 4 * kPageRegs, "a warpgroup would wait for registers");
+
+template <int D, bool SLAB, int NT>
+__global__ void __launch_bounds__(kPageThreads, 1) chunk_pages_kernel(const __grid_constant__ ChunkParams p) {
+  constexpr int kOperand = 128 * D * 2;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint8_t *q_tiles = smem, *tiles = smem + NT * kOperand, *ring = tiles + kPageSlots * kOperand;
+  ChunkShared &sh = *reinterpret_cast<ChunkShared *>(ring + kRawRing);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  chunk_begin(sh, NT, 4, 13);
   const uint32_t tmem = sh.tmem;
   grid_dependency_wait();
   allow_dependents_launch();
@@ -650,52 +710,327 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tiles_kernel(const __grid_c
   if (warp < 8) {
     const int x = warp >> 2, w = warp & 3;
     set_registers_up<kSoftmaxRegs>();
-    if (x < NT) {
-      load_rows<D>(p, view, b, kvh, x, w, lane, q_tiles + x * kOperand);
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&sh.bars.q_full));
-      chunk_softmax<D>(p, sh, view, b, kvh, x, w, lane, tmem);
-    }
+    if (x < NT) chunk_rows_role<D>(p, sh, view, b, kvh, x, w, lane, q_tiles + x * kOperand, tmem);
   } else if (warp < 12) {
     set_registers_down<kDequantRegs>();
     chunk_dequant<D, SLAB>(p, sh, ring, tiles, view, warp - 8, lane);
   } else {
     set_registers_down<kIssueRegs>();
     if (warp == 12) chunk_load<D>(p, sh, ring, view, b, kvh, lane);
-    if (warp == 13 && lane == 0) chunk_mma<D, NT>(p, sh, q_tiles, tiles, tmem);
+    if (warp == 13 && lane == 0) chunk_mma<D, NT, kPageSlots>(p, sh, q_tiles, tiles, tmem);
     __syncwarp();
   }
-  tc_fence_before();
-  __syncthreads();
-  if (warp == 13) {
-    tc_fence_after();
-    tmem_dealloc(tmem, kTmemCols);
+  chunk_end(tmem, 13);
+}
+
+// ==================================================== pages dequantised before
+// Where many row tiles share the pages, each page is dequantised once per call
+// into operand tiles in the workspace (plan, then unpack), and the attention
+// kernel copies whole tiles:
+//   counts [batch]                resident pages the call's rows may see
+//   lists  [batch][tiles * 8]     their descriptors, in order
+//   metas  [batch][tiles]         their columns and valid tokens
+//   tiles  [batch][kv head][tile] K tile, V tile
+struct __align__(16) PageList {  // of one tile, as the kernels read it: 64 bytes
+  int32_t col[kTilePages];
+  uint32_t page[kTilePages];
+};
+struct ChunkSpace {
+  int32_t *counts;
+  int64_t *lists;
+  PageList *metas;
+  uint8_t *tiles;
+  int32_t tiles_max;
+};
+
+// One CTA per sequence: the resident pages in column order.
+__global__ void __launch_bounds__(1024) chunk_plan_kernel(const __grid_constant__ ChunkParams p, const ChunkSpace w) {
+  __shared__ int warps[32];
+  grid_dependency_wait();
+  allow_dependents_launch();
+  const ChunkArgs &a = p.a;
+  const int b = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const ChunkView view = chunk_view(p, b, 0, p.rows_kv);
+  const int64_t *table = a.table + (int64_t)b * a.table_stride;
+  int64_t *list = w.lists + (int64_t)b * w.tiles_max * kTilePages;
+  PageList *metas = w.metas + (int64_t)b * w.tiles_max;
+  int n = 0;
+  for (int base = 0; base < view.total; base += 1024) {
+    const int v = base + (int)threadIdx.x;
+    int64_t d = 0;
+    int col = 0;
+    if (v < view.total) {
+      col = view.column(v);
+      d = __ldg(table + col);
+    }
+    const int mode = desc_mode(d);
+    bool ok = mode != AKV_MODE_SKIP;
+    if (ok && !page_in_arena(d, a.kv_heads * record_bytes(a.head_dim, 1 << a.log2_group, mode), a.arena_bytes)) {
+      set_status(a.status, AKV_DEV_BAD_DESCRIPTOR);
+      ok = false;
+    }
+    const uint32_t mask = __ballot_sync(0xffffffffu, ok);
+    if (lane == 0) warps[warp] = __popc(mask);
+    __syncthreads();
+    int before = 0, all = 0;
+    for (int i = 0; i < 32; ++i) {
+      if (i == warp) before = all;
+      all += warps[i];
+    }
+    __syncthreads();
+    if (ok) {
+      const int rank = n + before + __popc(mask & ((1u << lane) - 1u));
+      list[rank] = d;
+      metas[rank / kTilePages].col[rank % kTilePages] = col;
+      metas[rank / kTilePages].page[rank % kTilePages] = (uint32_t)mode | ((uint32_t)desc_ntok(d) << 2);
+    }
+    n += all;
   }
+  if (threadIdx.x < kTilePages && (int)threadIdx.x >= n % kTilePages && n % kTilePages) {
+    const int rank = n / kTilePages * kTilePages + (int)threadIdx.x;
+    list[rank] = 0;
+    metas[rank / kTilePages].col[threadIdx.x] = 0, metas[rank / kTilePages].page[threadIdx.x] = 0;
+  }
+  if (threadIdx.x == 0) w.counts[b] = n;
+}
+
+// One warp per (KV head, page, K or V) of a tile: 8 elements a lane and step, all
+// loads of a page issued before the first is converted.
+template <int D, bool SLAB>
+__global__ void __launch_bounds__(256) chunk_unpack_kernel(const __grid_constant__ ChunkParams p, const ChunkSpace w) {
+  constexpr int kOperand = 128 * D * 2, NC = D / 16, kUnits = D / 8, kRows = 32 / kUnits;
+  grid_dependency_wait();
+  allow_dependents_launch();
+  const ChunkArgs &a = p.a;
+  const int tile = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 31;
+  if (tile * kTilePages >= __ldcg(w.counts + b)) return;
+  const ChunkView view = chunk_view(p, b, 0, p.rows_kv);
+  const int64_t *list = w.lists + ((int64_t)b * w.tiles_max + tile) * kTilePages;
+  const int row0 = lane / kUnits, unit = lane % kUnits;
+  for (int job = blockIdx.z * 8 + (threadIdx.x >> 5); job < 2 * kTilePages * a.kv_heads; job += 8 * gridDim.z) {
+    const int kv = job & 1, i = (job >> 1) % kTilePages, kvh = (job >> 1) / kTilePages;
+    const int64_t d = __ldcg(list + i);
+    const int mode = desc_mode(d), ntok = desc_ntok(d);
+    const int pos0 = kBlock * __ldcg(&w.metas[(int64_t)b * w.tiles_max + tile].col[i]);
+    uint8_t *out = w.tiles + ((((int64_t)b * a.kv_heads + kvh) * w.tiles_max + tile) * 2 + kv) * kOperand;
+    const uint8_t *rec = a.arena + desc_offset(d) + kvh * record_bytes(D, 1 << a.log2_group, mode);
+    const int64_t pb = payload_bytes(D, mode);
+    const __half *sc = reinterpret_cast<const __half *>(rec + 2 * pb) + (kv ? (kBlock * D) >> a.log2_group : 0);
+    uint4 raw[NC];
+    float s[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) raw[c] = make_uint4(0u, 0u, 0u, 0u), s[c] = 0.f;
+    if (mode != AKV_MODE_SKIP) {
+      if (kv) slab_raw<D, NC, true>(mode, rec + pb, lane, raw);
+      else slab_raw<D, NC, false>(mode, rec, lane, raw);
+      if (mode != AKV_MODE_FP16) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) s[c] = __half2float(sc[SLAB ? 0 : (256 * c + 8 * lane) >> a.log2_group]);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int row = kRows * c + row0;
+      uint4 v = mode == AKV_MODE_SKIP ? raw[c] : raw8_to_f16(mode, raw[c], s[c]);
+      if (kv && (row >= ntok || !view.any(pos0 + row))) v = make_uint4(0u, 0u, 0u, 0u);
+      *reinterpret_cast<uint4 *>(out + panel_offset(kBlock * i + row, unit)) = v;
+    }
+  }
+}
+
+// The loader of whole tiles: 32 tiles' lists at a time, one per lane, a window
+// ahead; tiles that no row of the CTA sees are passed over.
+template <int D, int kSlots>
+__device__ __forceinline__ void chunk_load_tiles(const ChunkParams &p, const ChunkSpace &w, ChunkShared &sh,
+                                                 uint8_t *tiles, const ChunkView &view, int b, int kvh, int lane) {
+  constexpr int kOperand = 128 * D * 2;
+  const int pages = __ldcg(w.counts + b), count = (pages + kTilePages - 1) / kTilePages;
+  const PageList *metas = w.metas + (int64_t)b * w.tiles_max;
+  const uint8_t *src = w.tiles + ((int64_t)b * p.a.kv_heads + kvh) * w.tiles_max * 2 * kOperand;
+  uint4 next[4], cur[4];
+  auto fetch = [&](int w0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) next[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (w0 + lane < count) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) next[i] = __ldcg(reinterpret_cast<const uint4 *>(metas + w0 + lane) + i);
+    }
+  };
+  uint32_t mask = 0, wholes = 0;
+  int win0 = 0;
+  auto prepare = [&]() {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) cur[i] = next[i];
+    const uint32_t c[8] = {cur[0].x, cur[0].y, cur[0].z, cur[0].w, cur[1].x, cur[1].y, cur[1].z, cur[1].w};
+    const uint32_t g[8] = {cur[2].x, cur[2].y, cur[2].z, cur[2].w, cur[3].x, cur[3].y, cur[3].z, cur[3].w};
+    bool some = false, whole = true;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int col = (int)c[i], p0 = kBlock * col;
+      const bool here = (g[i] & 3u) != 0;
+      some |= here && p0 <= view.at_hi && (p0 + kBlock - 1 > view.at_lo - view.window || p0 < view.sinks);
+      whole &= here && (g[i] >> 2) == kBlock && view.whole_page(col);
+    }
+    mask = __ballot_sync(0xffffffffu, some);
+    wholes = __ballot_sync(0xffffffffu, whole);
+  };
+  fetch(0);
+  prepare();
+  fetch(32);
+  auto seek = [&]() {  // to the next window with a visible tile
+    while (mask == 0 && win0 + 32 < count) {
+      win0 += 32;
+      prepare();
+      fetch(win0 + 32);
+    }
+  };
+  seek();
+  if (mask == 0) {
+    if (lane == 0) {
+      sh.meta[0].last = 1, sh.meta[0].none = 1;
+      mbar_arrive(smem_u32(&sh.bars.kv_full[0]));
+    }
+    return;
+  }
+  for (int t = 0, n = 0;; ++t) {
+    const int k = __ffs(mask) - 1, tile = win0 + k;
+    TileMeta &m = sh.meta[t % kMetas];
+    // The first of this tile's slots is free only after the tile that last used
+    // its meta has been attended, so the wait comes before the writes.
+    const int slot = n % kSlots;
+    if (!mbar_wait_bounded(smem_u32(&sh.bars.kv_empty[slot]), ((n / kSlots) & 1) ^ 1)) break;
+    if (lane == k) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) reinterpret_cast<uint4 *>(&m)[i] = cur[i];
+      m.whole = (wholes >> k) & 1u;
+    }
+    mask &= mask - 1u;
+    seek();
+    const bool last = mask == 0;
+    if (lane == 0) m.last = last, m.none = 0;
+    __syncwarp();
+    bool ok = true;
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv, ++n) {
+      const int s = n % kSlots;
+      if (kv == 1) ok = mbar_wait_bounded(smem_u32(&sh.bars.kv_empty[s]), ((n / kSlots) & 1) ^ 1);
+      if (!ok) break;
+      if (lane == 0) {
+        const uint32_t bar = smem_u32(&sh.bars.kv_full[s]);
+        mbar_expect_tx(bar, kOperand);
+        bulk_g2s(smem_u32(tiles + s * kOperand), src + ((int64_t)tile * 2 + kv) * kOperand, kOperand, bar);
+      }
+    }
+    if (!ok) {  // the copies in flight end before the CTA does: its K tile's, at most
+      mbar_wait_bounded(smem_u32(&sh.bars.kv_full[slot]), ((n - 1) / kSlots) & 1);
+      break;
+    }
+    if (last) return;
+  }
+  if (lane == 0) set_status(p.a.status, AKV_DEV_TIMEOUT);
+}
+
+constexpr int kTileThreads = 384;
+// At launch, and after the split (softmax warpgroups; loader and MMA warpgroup).
+constexpr int kTileRegs = 168, kTileSoftmaxRegs = 216, kTileIssueRegs = 72;
+static_assert(2 * kTileSoftmaxRegs + kTileIssueRegs <= 3 * kTileRegs, "a warpgroup would wait for registers");
+template <int D>
+constexpr int tile_slots() {
+  return D == 128 ? 5 : 8;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kTileThreads, 1)
+    chunk_tiles_kernel(const __grid_constant__ ChunkParams p, const ChunkSpace w) {
+  constexpr int kOperand = 128 * D * 2, kSlots = tile_slots<D>();
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint8_t *q_tiles = smem, *tiles = smem + 2 * kOperand;
+  ChunkShared &sh = *reinterpret_cast<ChunkShared *>(tiles + kSlots * kOperand);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  chunk_begin(sh, 2, 1, 9);
+  const uint32_t tmem = sh.tmem;
+  grid_dependency_wait();
+  allow_dependents_launch();
+  const int kvh = blockIdx.y, b = blockIdx.z;
+  const int row0 = (int)blockIdx.x * 256;
+  const ChunkView view = chunk_view(p, b, row0, min(256, p.rows_kv - row0));
+  if (warp < 8) {
+    set_registers_up<kTileSoftmaxRegs>();
+    const int x = warp >> 2;
+    chunk_rows_role<D>(p, sh, view, b, kvh, x, warp & 3, lane, q_tiles + x * kOperand, tmem);
+  } else {
+    set_registers_down<kTileIssueRegs>();
+    if (warp == 8) chunk_load_tiles<D, kSlots>(p, w, sh, tiles, view, b, kvh, lane);
+    if (warp == 9 && lane == 0) chunk_mma<D, 2, kSlots>(p, sh, q_tiles, tiles, tmem);
+    __syncwarp();
+  }
+  chunk_end(tmem, 9);
+}
+
+// ------------------------------------------------------------------- host
+// Raise a kernel's shared-memory limit, once per device, and check that it starts
+// with the registers its warpgroups then share out.
+template <typename Kernel>
+static cudaError_t chunk_ready(Kernel kernel, int smem, int regs, std::atomic<bool> (&ready)[256]) {
+  int dev = 0;
+  if (cudaError_t err = cudaGetDevice(&dev)) return err;
+  if (dev < 256 && ready[dev].load(std::memory_order_acquire)) return cudaSuccess;
+  cudaFuncAttributes attr;
+  if (cudaError_t err = cudaFuncGetAttributes(&attr, kernel)) return err;
+  if (attr.numRegs != regs) return cudaErrorLaunchOutOfResources;
+  if (cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return err;
+  if (dev < 256) ready[dev].store(true, std::memory_order_release);
+  return cudaSuccess;
 }
 
 template <int D, bool SLAB, int NT>
-static cudaError_t chunk_launch(const ChunkParams &p) {
-  constexpr int smem = chunk_smem_bytes<D, NT>();
+static cudaError_t launch_pages(const ChunkParams &p) {
+  constexpr int smem = (NT + kPageSlots) * 128 * D * 2 + kRawRing + (int)sizeof(ChunkShared);
   static_assert(smem <= 232448, "one CTA's shared memory");
-  static std::atomic<bool> ready[256];  // per device ordinal
-  int dev = 0;
-  if (cudaError_t err = cudaGetDevice(&dev)) return err;
-  if (dev >= 256 || !ready[dev].load(std::memory_order_acquire)) {
-    // The warpgroups' register shares add up to kLaunchRegs a thread: the kernel has to start with that many.
-    cudaFuncAttributes attr;
-    if (cudaError_t err = cudaFuncGetAttributes(&attr, chunk_tiles_kernel<D, SLAB, NT>)) return err;
-    if (attr.numRegs != kLaunchRegs) return cudaErrorLaunchOutOfResources;
-    if (cudaError_t err = cudaFuncSetAttribute(chunk_tiles_kernel<D, SLAB, NT>,
-                                               cudaFuncAttributeMaxDynamicSharedMemorySize, smem))
-      return err;
-    if (dev < 256) ready[dev].store(true, std::memory_order_release);
-  }
+  static std::atomic<bool> ready[256];
+  if (cudaError_t err = chunk_ready(chunk_pages_kernel<D, SLAB, NT>, smem, kPageRegs, ready)) return err;
   const dim3 grid((p.rows_kv + 128 * NT - 1) / (128 * NT), p.a.kv_heads, p.a.batch);
-  return launch_dependent(chunk_tiles_kernel<D, SLAB, NT>, grid, kThreads, smem, p.a.stream, p);
+  return launch_dependent(chunk_pages_kernel<D, SLAB, NT>, grid, kPageThreads, smem, p.a.stream, p);
 }
 
-int chunk_tiles_launch(const ChunkArgs &a) {
+template <int D, bool SLAB>
+static cudaError_t launch_tiles(const ChunkParams &p, const ChunkSpace &w) {
+  constexpr int smem = (2 + tile_slots<D>()) * 128 * D * 2 + (int)sizeof(ChunkShared);
+  static_assert(smem <= 232448, "one CTA's shared memory");
+  static std::atomic<bool> ready[256];
+  if (cudaError_t err = chunk_ready(chunk_tiles_kernel<D>, smem, kTileRegs, ready)) return err;
+  cudaStream_t s = p.a.stream;
+  if (cudaError_t err = launch_dependent(chunk_plan_kernel, p.a.batch, 1024, 0, s, p, w)) return err;
+  if (w.tiles_max > 0)
+    if (cudaError_t err = launch_dependent(chunk_unpack_kernel<D, SLAB>, dim3(w.tiles_max, p.a.batch, 2), 256, 0, s, p, w))
+      return err;
+  const dim3 grid((p.rows_kv + 255) / 256, p.a.kv_heads, p.a.batch);
+  return launch_dependent(chunk_tiles_kernel<D>, grid, kTileThreads, smem, s, p, w);
+}
+
+// Tiles the rows of a call may see, at most.
+static int64_t space_tiles(const ChunkArgs &a) {
+  int64_t columns = a.columns;
+  if (a.window < (1 << 30)) columns = std::min<int64_t>(columns, a.lead + ((int64_t)a.window + a.rows + 2 * kBlock - 3) / kBlock);
+  return (columns + kTilePages - 1) / kTilePages;
+}
+static int64_t align256(int64_t n) { return (n + 255) & ~(int64_t)255; }
+static int64_t space_layout(const ChunkArgs &a, int64_t tiles, uint8_t *base, ChunkSpace *w) {
+  const int64_t counts = 0, lists = align256(4ll * a.batch);
+  const int64_t metas = lists + align256(8ll * kTilePages * tiles * a.batch);
+  const int64_t data = (metas + align256((int64_t)sizeof(PageList) * tiles * a.batch) + 1023) & ~(int64_t)1023;
+  if (w) {
+    w->counts = (int32_t *)(base + counts), w->lists = (int64_t *)(base + lists);
+    w->metas = (PageList *)(base + metas), w->tiles = base + data, w->tiles_max = (int32_t)tiles;
+  }
+  return data + tiles * a.batch * a.kv_heads * 2 * 128 * a.head_dim * 2;
+}
+
+int64_t chunk_tiles_bytes(const ChunkArgs &a) {
+  return a.rows * (a.q_heads / a.kv_heads) > 128 ? space_layout(a, space_tiles(a), nullptr, nullptr) : 0;
+}
+
+int chunk_tiles_launch(const ChunkArgs &a, void *workspace, int64_t workspace_bytes) {
   ChunkParams p;
   p.a = a;
   p.heads_per_kv = a.q_heads / a.kv_heads;
@@ -704,14 +1039,19 @@ int chunk_tiles_launch(const ChunkArgs &a) {
   p.q_sign = a.scale > 0.f ? 1 : (a.scale < 0.f ? -1 : 0);
   p.scale_log2 = p.q_sign == 0 ? 1.f : fabsf(a.scale) * 1.4426950408889634f;
   p.vector_out = ((uintptr_t)a.out & 15) == 0 && a.o_bs % 8 == 0 && a.o_hs % 8 == 0 && a.o_ts % 8 == 0;
-  const bool slab = (1 << a.log2_group) == 16 * a.head_dim, two = p.rows_kv > 128;
+  const bool slab = (1 << a.log2_group) == 16 * a.head_dim;
+  const int64_t need = chunk_tiles_bytes(a);
   cudaError_t err;
-  if (a.head_dim == 64)
-    err = slab ? (two ? chunk_launch<64, true, 2>(p) : chunk_launch<64, true, 1>(p))
-               : (two ? chunk_launch<64, false, 2>(p) : chunk_launch<64, false, 1>(p));
-  else
-    err = slab ? (two ? chunk_launch<128, true, 2>(p) : chunk_launch<128, true, 1>(p))
-               : (two ? chunk_launch<128, false, 2>(p) : chunk_launch<128, false, 1>(p));
+  if (need > 0) {
+    if (workspace_bytes < need) return AKV_ERR_INVALID;
+    ChunkSpace w;
+    space_layout(a, space_tiles(a), (uint8_t *)workspace, &w);
+    if (a.head_dim == 64) err = slab ? launch_tiles<64, true>(p, w) : launch_tiles<64, false>(p, w);
+    else err = slab ? launch_tiles<128, true>(p, w) : launch_tiles<128, false>(p, w);
+  } else {
+    if (a.head_dim == 64) err = slab ? launch_pages<64, true, 1>(p) : launch_pages<64, false, 1>(p);
+    else err = slab ? launch_pages<128, true, 1>(p) : launch_pages<128, false, 1>(p);
+  }
   return err == cudaSuccess ? AKV_OK : AKV_ERR_CUDA;
 }
 

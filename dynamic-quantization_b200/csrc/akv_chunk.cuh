@@ -26,6 +26,8 @@ struct ChunkArgs {
   cudaStream_t stream;
 };
 
-int chunk_tiles_launch(const ChunkArgs &a);
+// Bytes of workspace the call needs (0: none).
+int64_t chunk_tiles_bytes(const ChunkArgs &a);
+int chunk_tiles_launch(const ChunkArgs &a, void *workspace, int64_t workspace_bytes);
 
 }  // namespace akv

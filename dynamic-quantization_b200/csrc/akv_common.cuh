@@ -64,6 +64,85 @@ __host__ __device__ constexpr int64_t v_swizzle(int D, int mode, int64_t o) {
   return mode == AKV_MODE_SKIP ? o : o ^ ((int64_t)v_swizzle_key(D * mode_bits(mode) / 8, o) << 4);
 }
 
+// Byte XOR that turns the row-major offset of a lane's 8 elements of chunk c
+// (elements 256c + 8 lane of a [16][D] slab) into their stored offset in a V
+// payload: v_swizzle with the key worked out for these offsets (it depends on
+// c alone for head_dim 128, on c and the lane for head_dim 64).
+template <int D>
+__device__ __forceinline__ int v_chunk_xor(int mode, int c, int lane) {
+  int key;
+  if constexpr (D == 128)
+    key = mode == AKV_MODE_FP16 ? ((c & 1) | ((c & 2) << 1)) : ((2 * c) & 6);
+  else
+    key = mode == AKV_MODE_INT4 ? ((2 * c) & 2) : (((4 * c) & 4) | ((lane >> 3) & 2));
+  return key << 4;
+}
+
+// The payload bytes of 8 consecutive elements (e = 256 c + 8 lane) of a record:
+// FP16 all 16 bytes, INT8 8 bytes in .x / .y, INT4 4 bytes in .x.  `VPAY`: a V
+// payload, stored in the swizzled byte order (v_swizzle).
+template <int D, bool VPAY>
+__device__ __forceinline__ uint4 record_raw8(int mode, const uint8_t *payload, int c, int lane) {
+  const int e = 256 * c + 8 * lane;
+  const int vx = VPAY ? v_chunk_xor<D>(mode, c, lane) : 0;
+  if (mode == AKV_MODE_FP16) return *reinterpret_cast<const uint4 *>(payload + ((2 * e) ^ vx));
+  if (mode == AKV_MODE_INT8) {
+    const uint2 w = *reinterpret_cast<const uint2 *>(payload + (e ^ vx));
+    return make_uint4(w.x, w.y, 0u, 0u);
+  }
+  return make_uint4(*reinterpret_cast<const uint32_t *>(payload + ((e / 2) ^ vx)), 0u, 0u, 0u);
+}
+
+// record_raw8 for all NC chunks of a slab, the mode tested once: the loads form
+// one straight-line batch.
+template <int D, int NC, bool VPAY>
+__device__ __forceinline__ void slab_raw(int mode, const uint8_t *payload, int lane, uint4 (&raw)[NC]) {
+  if (mode == AKV_MODE_FP16) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) raw[c] = record_raw8<D, VPAY>(AKV_MODE_FP16, payload, c, lane);
+  } else if (mode == AKV_MODE_INT8) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) raw[c] = record_raw8<D, VPAY>(AKV_MODE_INT8, payload, c, lane);
+  } else {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) raw[c] = record_raw8<D, VPAY>(AKV_MODE_INT4, payload, c, lane);
+  }
+}
+
+// The 8 integers of a raw INT8 / INT4 chunk.
+__device__ __forceinline__ void raw8_ints(int mode, uint4 w, int (&q)[8]) {
+  if (mode == AKV_MODE_INT8) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      q[i] = (int)(int8_t)(w.x >> (8 * i));
+      q[4 + i] = (int)(int8_t)(w.y >> (8 * i));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int n = (w.x >> (4 * i)) & 15;
+      q[i] = n >= 8 ? n - 16 : n;
+    }
+  }
+}
+
+// A raw chunk dequantized to fp16 exactly as QuantizedPage.dense
+// (packed_decode.py:34-45): fp16(int * float(scale)), `s` the element group's
+// scale (unused for FP16 pages).
+__device__ __forceinline__ uint4 raw8_to_f16(int mode, uint4 w, float s) {
+  if (mode == AKV_MODE_FP16) return w;
+  int q[8];
+  raw8_ints(mode, w, q);
+  uint32_t h[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half lo = __float2half_rn((float)q[2 * i] * s);
+    const __half hi = __float2half_rn((float)q[2 * i + 1] * s);
+    h[i] = (uint32_t)__half_as_ushort(lo) | ((uint32_t)__half_as_ushort(hi) << 16);
+  }
+  return make_uint4(h[0], h[1], h[2], h[3]);
+}
+
 // ------------------------------------------------------------------ PTX: sync
 __device__ __forceinline__ uint32_t smem_u32(const void *p) {
   return (uint32_t)__cvta_generic_to_shared(p);

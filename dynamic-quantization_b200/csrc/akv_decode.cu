@@ -1747,7 +1747,12 @@ extern "C" int64_t akv_chunk_workspace_bytes(int32_t batch, int32_t rows, int32_
   ChunkPlan c;
   Plan pl;
   if (chunk_plan(batch, rows, q_heads, kv_heads, head_dim, max_blocks, window, sinks, &c) != AKV_OK) return -1;
-  if (use_tiles(rows * c.rows.heads_per_kv)) return kHeaderBytes;
+  if (use_tiles(rows * c.rows.heads_per_kv)) {
+    ChunkArgs a = {};
+    a.columns = max_blocks, a.batch = batch, a.rows = rows, a.q_heads = q_heads, a.kv_heads = kv_heads;
+    a.head_dim = head_dim, a.window = c.rows.window, a.lead = c.rows.lead;
+    return std::max(kHeaderBytes, chunk_tiles_bytes(a));
+  }
   if (make_plan(batch, c.rows_total, kv_heads, head_dim, c.columns, splits, &pl) != AKV_OK) return -1;
   return pl.smax > kMaxSegments ? -1 : pl.bytes;
 }
@@ -1768,7 +1773,7 @@ extern "C" int akv_chunk_attention(const void *arena, int64_t arena_bytes, const
   c.rows.q_ts = q_token_stride;
   cudaStream_t s = (cudaStream_t)stream;
   if (use_tiles(rows * c.rows.heads_per_kv)) {
-    if (!arena || !table || !query || table_stride < max_blocks || arena_bytes < 0 || !isfinite(scale)) return AKV_ERR_INVALID;
+    if (!arena || !table || !query || !workspace || ((uintptr_t)workspace & 15) || table_stride < max_blocks || arena_bytes < 0 || !isfinite(scale)) return AKV_ERR_INVALID;
     if (((uintptr_t)arena & 15) || ((uintptr_t)query & 15) || q_batch_stride % 8 || q_head_stride % 8) return AKV_ERR_INVALID;
     const int lg = ilog2_exact(group);
     if (lg < 0 || (group != 32 && group != 64 && group != 128 && group != 16 * head_dim)) return AKV_ERR_UNSUPPORTED;
@@ -1780,7 +1785,7 @@ extern "C" int akv_chunk_attention(const void *arena, int64_t arena_bytes, const
     a.batch = batch, a.rows = rows, a.q_heads = q_heads, a.kv_heads = kv_heads, a.head_dim = head_dim;
     a.log2_group = lg, a.window = c.rows.window, a.sinks = c.rows.sinks, a.lead = c.rows.lead;
     a.scale = scale, a.status = dev_status, a.stream = s;
-    return chunk_tiles_launch(a);
+    return chunk_tiles_launch(a, workspace, workspace_bytes);
   }
   if (int st = decode_launch(arena, arena_bytes, table, table_stride, seq_blocks, c.columns, query, q_batch_stride,
                              q_head_stride, batch, c.rows_total, kv_heads, head_dim, group, scale, splits, workspace,
