@@ -1,8 +1,8 @@
 // Chunk attention on the 5th-generation tensor cores (tcgen05, TMEM).
 //
-// The rows of a KV head are its (query token, query head) pairs, token-major.  A
-// CTA holds one or two tiles of 128 rows and walks the pages they can see in
-// tiles of 128 tokens (8 resident pages; evicted pages take no place in a tile):
+// The rows of a KV head are its (query token, query head) pairs, token-major; 128 of
+// them form a row tile.  The pages that the rows can see are walked in tiles of
+// 128 tokens (8 resident pages; evicted pages take no place in a tile):
 //
 //   S = Q K^T          tcgen05.mma, both operands in shared memory, S in TMEM
 //   P = 2^(c S - m)    one thread per row: running max m and sum l in fp32
@@ -12,11 +12,12 @@
 // V's values are fp16; m moves only when a tile exceeds it by 2^8 (then O is
 // rescaled), so P <= 2^8 and its rounding is relative, 2^-11 a term.
 //
-// Roles (warps): 0-3 and 4-7 softmax of the two row tiles; 8-11 dequantise pages
-// into operand tiles; 12 loads records (bulk copies into a byte ring); 13 issues
-// the MMAs.  K and V are dequantised to the values the reference attends over,
-// fp16(int * float(scale)), once per CTA and tile.  Waits are bounded: a role whose
-// wait runs out reports AKV_DEV_TIMEOUT and leaves its loop.
+// A page would be dequantised once per pair of row tiles; chunk_unpack_kernel does it
+// once per call instead, into operand tiles in the workspace, and the attention
+// kernel copies whole tiles.  It runs one CTA per SM, each with two row tiles that
+// share every K and V tile; the work (row tiles x tiles of tokens) is cut into equal
+// contiguous ranges, one per CTA, whose partial (O, m, l) a merge kernel joins.
+// Waits are bounded: a role whose wait runs out reports AKV_DEV_TIMEOUT and leaves.
 #include <math.h>
 #include <stddef.h>
 
@@ -73,33 +74,25 @@ __device__ __forceinline__ void tc_ld32(uint32_t addr, float *v) {
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(addr));
 }
-__device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t *r) {
+__device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t *r) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
-      "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
       "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
-      "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
-      "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(addr)
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr)
       : "memory");
 }
-// Shared memory by 32-bit address.
-__device__ __forceinline__ uint32_t lds32(uint32_t a) {
-  uint32_t v;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
-  return v;
-}
-__device__ __forceinline__ void lds64(uint32_t a, uint32_t (&v)[2]) {
-  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(a) : "memory");
-}
-__device__ __forceinline__ void lds128(uint32_t a, uint32_t (&v)[4]) {
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
-               : "r"(a)
+__device__ __forceinline__ void tc_st8(uint32_t addr, const uint32_t *r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(addr)
                : "memory");
 }
-__device__ __forceinline__ void sts128(uint32_t a, const uint32_t (&v)[4]) {
-  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+__device__ __forceinline__ void tc_ld16(uint32_t addr, float *v) {
+  uint32_t *r = reinterpret_cast<uint32_t *>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
 }
 template <int N>
 __device__ __forceinline__ void set_registers_up() {
@@ -132,42 +125,65 @@ constexpr uint32_t mma_idesc(int n, bool b_mn_major) {
 
 constexpr int kTilePages = 8;
 constexpr int kTileTokens = kTilePages * kBlock;
-constexpr int kMaxSlots = 8;    // operand tiles: K0 V0 K1 V1 ...
-constexpr int kItems = 8;       // half tiles of raw records in flight
-constexpr int kMetas = 8;       // the loader runs at most 5 tiles ahead of the softmax
-constexpr int kRawRing = 32768;
+constexpr int kMaxSlots = 8;  // operand tiles: K0 V0 K1 V1 ...
 constexpr int kTmemCols = 512;
-constexpr uint32_t kTmemS = 0, kTmemO = 256;  // S/P of row tile x at 128 x, O at 256 + 128 x
+constexpr uint32_t kTmemS = 0, kTmemO = 256;  // S/P of stream x at 128 x, O at 256 + 128 x
 
+// What the roles have to know about a tile of tokens.
 struct __align__(16) TileMeta {
   int32_t col[kTilePages];
   uint32_t page[kTilePages];  // mode | valid tokens << 2; 0: no page
-  int64_t src[kTilePages];    // byte offset of the KV head's record (page kernel)
-  uint32_t last, whole, none;  // no tile follows; every row of the CTA sees every token; there is no tile at all
+  uint32_t last;              // no tile of this segment follows
+  uint32_t whole;             // every row of the CTA sees every token
+  uint32_t none;              // not a tile: the segment has none
+  uint32_t pad;
+};
+struct __align__(16) PageList {  // a tile's part that chunk_plan_kernel writes
+  int32_t col[kTilePages];
+  uint32_t page[kTilePages];
 };
 
 struct ChunkBars {
-  uint64_t raw_full[kItems], raw_empty[kItems], kv_full[kMaxSlots], kv_empty[kMaxSlots], q_full, s_full[2], p_full[2],
-      o_full[2];
+  uint64_t kv_full[kMaxSlots], kv_empty[kMaxSlots], q_full[2], s_full[2], p_full[2], o_full[2];
 };
-
+// Where a CTA's range of the work begins.
+struct Place {
+  int32_t b, kvh, m, pos;  // sequence, KV head, row block, tile within the unit
+  int64_t left;            // tiles of the range
+};
+template <int D>
 struct ChunkShared {
+  // The loader is at most as many metas ahead as there are slots.
+  static constexpr int kSlots = D == 128 ? 5 : 8, kMetas = D == 128 ? 8 : 16;
   ChunkBars bars;
   TileMeta meta[kMetas];
-  uint32_t raw_at[kItems][4];  // ring offset of each page of an item
+  Place place;
   uint32_t tmem;
+  float shared_rows[2][2][128];  // [stream][half][row]: what the two threads of a row exchange
 };
+static_assert(sizeof(ChunkBars) % 16 == 0 && sizeof(TileMeta) % 16 == 0, "lists move 16 bytes at a time");
 
-
-static_assert(offsetof(ChunkShared, meta) % 16 == 0 && sizeof(TileMeta) % 16 == 0, "lists move 16 bytes at a time");
-
+// What the tiles kernel reads from the workspace.
+struct ChunkSpace {
+  int32_t *counts;   // [batch]: resident pages that the call's rows may see
+  int64_t *lists;    // [batch][tiles_max * 8]: their descriptors, in order
+  PageList *metas;   // [batch][tiles_max]: their columns and valid tokens
+  int4 *ranges;      // [batch][blocks]: sink tiles, first window tile, tiles
+  int32_t *prefix;   // [batch][blocks + 1]: tiles of the row blocks before
+  int4 *cuts;        // [CTAs]: what its range cut (see chunk_merge_kernel)
+  uint8_t *tiles;    // [batch][kv head][tiles_max]: K tile, V tile
+  int32_t tiles_max;
+};
 struct ChunkParams {
   ChunkArgs a;
-  int32_t heads_per_kv, rows_kv, q_sign, vector_out;
+  int32_t heads_per_kv, rows_kv, blocks, q_sign, vector_out, ctas;
+  FastDiv fd_hpk;  // heads_per_kv
   float scale_log2;
+  float *partials;  // rows of D + 4: O, m, l
+  ChunkSpace w;
 };
 
-// What a CTA's rows see: rows row0 .. row0 + n - 1 of a KV head.
+// What a block of rows sees: rows row0 .. row0 + n - 1 of a KV head.
 struct ChunkView {
   int at_first, row0, n, at_lo, at_hi, window, sinks;
   int lead, first, total;  // virtual page columns: 0 .. lead - 1, then first ..; `total` of them
@@ -187,8 +203,8 @@ __device__ __forceinline__ ChunkView chunk_view(const ChunkParams &p, int b, int
   const int tokens = min(a.tokens ? __ldg(a.tokens + b) : a.uniform_tokens, kBlock * held);
   v.at_first = tokens - a.rows;
   v.row0 = row0, v.n = nrows;
-  v.at_lo = v.at_first + row0 / p.heads_per_kv;
-  v.at_hi = v.at_first + (row0 + nrows - 1) / p.heads_per_kv;
+  v.at_lo = v.at_first + fdiv(row0, p.fd_hpk);
+  v.at_hi = v.at_first + fdiv(row0 + nrows - 1, p.fd_hpk);
   v.window = a.window, v.sinks = a.sinks, v.lead = a.lead;
   v.first = max(a.lead, max(v.at_lo - a.window + 1, 0) / kBlock);
   const int end = v.at_hi < 0 ? 0 : min(v.at_hi / kBlock + 1, held);  // columns up to the newest row's
@@ -196,316 +212,263 @@ __device__ __forceinline__ ChunkView chunk_view(const ChunkParams &p, int b, int
   return v;
 }
 
-// ------------------------------------------------------------------ loader
-// Descriptors are read 32 columns at a time, one per lane, a window ahead; the
-// resident pages of a window fill tiles in order.
-template <int D>
-__device__ __forceinline__ void chunk_load(const ChunkParams &p, ChunkShared &sh, uint8_t *ring, const ChunkView &view,
-                                           int b, int kvh, int lane) {
-  const ChunkArgs &a = p.a;
-  const uint32_t scale_bytes = 2u * (uint32_t)((kBlock * D) >> a.log2_group);  // K's (or V's) scales of a record
-  const int64_t *table = a.table + (int64_t)b * a.table_stride;
-  auto fetch = [&](int w0, int64_t &raw, int &col) {
-    const int v = w0 + lane;
-    raw = 0, col = 0;
-    if (v < view.total) {
-      col = view.column(v);
-      raw = __ldg(table + col);
-    }
-  };
-  int64_t src = 0;
-  uint32_t page = 0, mask = 0;
-  int col = 0;
-  auto prepare = [&](int64_t raw, int c) {
-    const int mode = desc_mode(raw);
-    bool ok = mode != AKV_MODE_SKIP;
-    int64_t rb = 2 * payload_bytes(D, mode) + (mode == AKV_MODE_FP16 ? 0 : 2 * (int64_t)scale_bytes);
-    rb = (rb + 15) & ~(int64_t)15;
-    if (ok && !page_in_arena(raw, rb * a.kv_heads, a.arena_bytes)) {
-      set_status(a.status, AKV_DEV_BAD_DESCRIPTOR);
-      ok = false;
-    }
-    src = desc_offset(raw) + kvh * rb;
-    page = (uint32_t)mode | ((uint32_t)desc_ntok(raw) << 2);
-    col = c;
-    mask = __ballot_sync(0xffffffffu, ok);
-  };
-  int win0 = 0, next_col;
-  int64_t next_raw;
-  {
-    int64_t raw;
-    int c;
-    fetch(0, raw, c);
-    fetch(32, next_raw, next_col);
-    prepare(raw, c);
+// ------------------------------------------------------------ work of a CTA
+// Units are (sequence, KV head, row block), the row block fastest; a unit's cost is
+// its tiles of tokens, at least 1 (its rows are written all the same).  The costs
+// laid end to end are cut into equal ranges.
+struct TileWork {  // as chunk_plan_kernel found it
+  const ChunkParams &p;
+  __device__ __forceinline__ int before(int b, int m) const {
+    return __ldcg(p.w.prefix + (int64_t)b * (p.blocks + 1) + m);
   }
-  auto advance = [&]() {
-    win0 += 32;
-    const int64_t raw = next_raw;
-    const int c = next_col;
-    fetch(win0 + 32, next_raw, next_col);
-    prepare(raw, c);
-  };
-
-  uint32_t head = 0, head_p = 0, tail = 0;  // byte ring: virtual positions and the physical write position
-  uint32_t starts = 0;                      // lane i: virtual start of the item in slot i
-  int issued = 0, freed = 0;
-  bool dead = false;
-  for (int tile = 0; !dead; ++tile) {
-    TileMeta &m = sh.meta[tile % kMetas];
-    int have = 0;
-    while (have < kTilePages) {
-      if (mask == 0) {
-        if (win0 + 32 >= view.total) break;
-        advance();
-        continue;
-      }
-      const int rank = have + __popc(mask & ((1u << lane) - 1u));
-      const bool take = ((mask >> lane) & 1u) && rank < kTilePages;
-      if (take) m.col[rank] = col, m.page[rank] = page, m.src[rank] = src;
-      const uint32_t taken = __ballot_sync(0xffffffffu, take);
-      mask &= ~taken;
-      have += __popc(taken);
-    }
-    if (lane >= have && lane < kTilePages) m.col[lane] = 0, m.page[lane] = 0, m.src[lane] = 0;
-    while (mask == 0 && win0 + 32 < view.total) advance();
-    const bool last = mask == 0;
-    __syncwarp();
-    bool whole = true;
-    if (lane < kTilePages) whole = (m.page[lane] >> 2) == kBlock && view.whole_page(m.col[lane]);
-    whole = __all_sync(0xffffffffu, whole);
-    if (lane == 0) m.last = last, m.whole = whole, m.none = 0;
-    __syncwarp();
-    for (int part = 0; part < 4; ++part) {  // K of pages 0-3, of 4-7, then V
-      const int kv = part >> 1, i = 4 * (part & 1) + (lane & 3);
-      const int mode = lane < 4 ? (int)(m.page[i] & 3) : 0;
-      const uint32_t pay = mode ? (uint32_t)payload_bytes(D, mode) : 0u;
-      // K and V scales lie one after the other; both of a slab record share one 16-byte unit
-      const uint32_t sc = mode == 0 || mode == AKV_MODE_FP16 ? 0u : max(16u, scale_bytes);
-      uint32_t off = pay + sc;
+  __device__ __forceinline__ int cost(int b, int m) const { return before(b, m + 1) - before(b, m); }
+  __device__ __forceinline__ int total(int b) const { return before(b, p.blocks); }
+};
+__device__ __forceinline__ int64_t warp_sum(int64_t v) {
 #pragma unroll
-      for (int d = 1; d < 4; d <<= 1) {
-        const uint32_t o = __shfl_up_sync(0xffffffffu, off, d);
-        if (lane >= d) off += o;
-      }
-      const uint32_t total = __shfl_sync(0xffffffffu, off, 3);
-      off -= pay + sc;
-      const int slot = issued % kItems;
-      uint32_t start, start_p;
-      while (true) {
-        start = head, start_p = head_p;
-        if (issued == freed && start_p != 0) {  // empty ring: restart at a lap boundary
-          start += kRawRing - start_p;
-          start_p = 0;
-          tail = start;
-        } else if (start_p + total > (uint32_t)kRawRing) {
-          start += kRawRing - start_p;
-          start_p = 0;
-        }
-        if (issued - freed < kItems && start + total - tail <= (uint32_t)kRawRing) break;
-        if (!mbar_wait_bounded(smem_u32(&sh.bars.raw_empty[freed % kItems]), (freed / kItems) & 1)) {
-          dead = true;
-          break;
-        }
-        ++freed;
-        tail = freed == issued ? head : __shfl_sync(0xffffffffu, starts, freed % kItems);
-      }
-      if (dead) break;
-      if (lane == slot) starts = start;
-      if (lane < 4) sh.raw_at[slot][lane] = start_p + off;
-      __syncwarp();
-      const uint32_t bar = smem_u32(&sh.bars.raw_full[slot]);
-      if (lane == 0) mbar_expect_tx(bar, total);
-      __syncwarp();
-      if (mode) {
-        const uint8_t *rec = a.arena + m.src[i];
-        const uint32_t dst = smem_u32(ring + start_p + off);
-        bulk_g2s(dst, rec + kv * pay, pay, bar);
-        if (sc) bulk_g2s(dst + pay, rec + 2 * pay + (kv && scale_bytes >= 16 ? scale_bytes : 0), sc, bar);
-      }
-      head = start + total, head_p = start_p + total;
-      ++issued;
-    }
-    if (last) break;
-  }
-  if (dead) {
-    if (lane == 0) set_status(a.status, AKV_DEV_TIMEOUT);
-    for (int i = freed; i < issued; ++i)  // let the copies in flight land (bounded)
-      if (!mbar_wait_bounded(smem_u32(&sh.bars.raw_full[i % kItems]), (i / kItems) & 1)) break;
-  }
+  for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  return v;
 }
-
-// ------------------------------------------------------------ dequantisation
-// One page's K or V payload (at raw, scales behind it) into tokens token0 .. + 15
-// of an operand tile, by one warp: 8 elements (one 16-byte unit of the tile) a
-// lane and step.  `seen(row)`: V rows that no row sees become zero, so that a
-// weight of 0 never meets what their memory holds.
-template <int D, int MODE, bool VPAY, bool SLAB, typename Seen>
-__device__ __forceinline__ void dequant_page(const uint8_t *raw, const __half *scales, int log2_group, uint8_t *tile,
-                                             int token0, int lane, bool check, Seen seen) {
-  constexpr int NC = D / 16;
-  constexpr int BYTES = MODE == AKV_MODE_FP16 ? 16 : (MODE == AKV_MODE_INT8 ? 8 : 4);  // of 8 elements
-  // Chunk c holds elements 256 c + 8 lane + [0, 8): row kRows c + row0, unit `unit`.
-  // Both swizzles are XORs of bits that c alone (or c and the lane apart) sets, so
-  // an address is a lane constant, one XOR with a constant and an immediate.
-  constexpr int kUnits = D / 8, kRows = 32 / kUnits;
-  const int row0 = lane / kUnits, unit = lane % kUnits;
-  const uint32_t dst0 = smem_u32(tile) + (uint32_t)((unit >> 3) * kPanel + (token0 + row0) * 128 + (((unit & 7) ^ row0) << 4));
-  const uint32_t src0 = smem_u32(raw);
-  const __half *sc = SLAB ? scales : scales + ((8 * lane) >> log2_group);
+// All of the work, by a whole warp.
+__device__ __forceinline__ int64_t work_total(const TileWork &work) {
+  const ChunkArgs &a = work.p.a;
+  int64_t all = 0;
+  for (int b = threadIdx.x & 31; b < a.batch; b += 32) all += (int64_t)work.total(b) * a.kv_heads;
+  return warp_sum(all);
+}
+// A range of fewer tiles than this costs more to set up than it saves.
+constexpr int kMinTiles = 2;
+__device__ __forceinline__ int work_ctas(const ChunkParams &p, int64_t all) {
+  return (int)max((int64_t)1, min((int64_t)p.ctas, (all + kMinTiles - 1) / kMinTiles));
+}
+__device__ __forceinline__ int64_t range_start(int64_t all, int ctas, int c) { return all * c / ctas; }
+__device__ __forceinline__ Place find_place(const TileWork &work, int cta) {  // a whole warp
+  const ChunkArgs &a = work.p.a;
+  const int lane = threadIdx.x & 31;
+  const int64_t all = work_total(work);
+  const int ctas = work_ctas(work.p, all);
+  Place at{0, 0, 0, 0, 0};
+  if (cta >= ctas) return at;
+  int64_t start = range_start(all, ctas, cta);
+  at.left = range_start(all, ctas, cta + 1) - start;
+  for (int b0 = 0;; b0 += 32) {  // the sequence
+    const int64_t t = b0 + lane < a.batch ? (int64_t)work.total(b0 + lane) * a.kv_heads : 0;
+    int64_t upto = t;
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    const uint32_t src = src0 + (uint32_t)((BYTES * lane) ^ (VPAY ? v_chunk_xor<D>(MODE, c, lane) : 0)) + 32 * BYTES * c;
-    uint32_t h[4];
-    if constexpr (MODE == AKV_MODE_FP16) {
-      lds128(src, h);
-    } else {
-      const uint32_t s1 = __half_as_ushort(sc[SLAB ? 0 : (256 * c) >> log2_group]), s = s1 | (s1 << 16);
-      if constexpr (MODE == AKV_MODE_INT8) {
-        uint32_t w[2];
-        lds64(src, w);
-        h[0] = hmul2(int8_to_f16x2(prmt(w[0], 0, 0x1100)), s), h[1] = hmul2(int8_to_f16x2(prmt(w[0], 0, 0x3322)), s);
-        h[2] = hmul2(int8_to_f16x2(prmt(w[1], 0, 0x1100)), s), h[3] = hmul2(int8_to_f16x2(prmt(w[1], 0, 0x3322)), s);
-      } else {
-        const uint32_t w = lds32(src);
-        const uint32_t e04 = hmul2(int4_lo_to_f16x2(w), s), e15 = hmul2(int4_hi_to_f16x2(w), s);
-        const uint32_t e26 = hmul2(int4_lo_to_f16x2(w >> 8), s), e37 = hmul2(int4_hi_to_f16x2(w >> 8), s);
-        h[0] = prmt(e04, e15, 0x5410), h[1] = prmt(e26, e37, 0x5410);
-        h[2] = prmt(e04, e15, 0x7632), h[3] = prmt(e26, e37, 0x7632);
-      }
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t o = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += o;
     }
-    if (VPAY && check && !seen(kRows * c + row0)) h[0] = h[1] = h[2] = h[3] = 0u;
-    sts128((dst0 ^ (((kRows * c) & 7) << 4)) + kRows * 128 * c, h);
-  }
-}
-
-template <int D, bool SLAB>
-__device__ __forceinline__ void chunk_dequant(const ChunkParams &p, ChunkShared &sh, const uint8_t *ring, uint8_t *tiles,
-                                              const ChunkView &view, int warp, int lane) {
-  constexpr int kOperand = 128 * D * 2;
-  constexpr int kSlots = 4;
-  const int lg = p.a.log2_group;
-  bool dead = false;
-  for (int n = 0; !dead; ++n) {
-    const int slot = n % kSlots, kv = n & 1;
-    const TileMeta &m = sh.meta[(n >> 1) % kMetas];
-    uint8_t *tile = tiles + slot * kOperand;
-    if (!mbar_wait_bounded(smem_u32(&sh.bars.kv_empty[slot]), ((n / kSlots) & 1) ^ 1)) {
-      dead = true;
+    const uint32_t hit = __ballot_sync(0xffffffffu, start < upto);
+    if (hit) {
+      const int k = __ffs(hit) - 1;
+      at.b = b0 + k;
+      start -= __shfl_sync(0xffffffffu, upto - t, k);
       break;
     }
-    for (int half = 0; half < 2; ++half) {
-      const int item = 2 * n + half, rs = item % kItems, i = 4 * half + warp;
-      if (!mbar_wait_bounded(smem_u32(&sh.bars.raw_full[rs]), (item / kItems) & 1)) {
-        dead = true;
-        break;
+    start -= __shfl_sync(0xffffffffu, upto, 31);
+  }
+  const int per_head = work.total(at.b);
+  at.kvh = (int)(start / per_head);
+  const int rest = (int)(start - (int64_t)at.kvh * per_head);
+  int m = 0;  // the row block: the last whose `before` is at most rest
+  for (int m0 = 0; m0 < work.p.blocks; m0 += 32) {
+    const bool upto = m0 + lane < work.p.blocks && work.before(at.b, m0 + lane) <= rest;
+    const uint32_t hit = __ballot_sync(0xffffffffu, upto);
+    if (hit) m = m0 + 31 - __clz(hit);
+    if (hit != 0xffffffffu) break;
+  }
+  at.m = m, at.pos = rest - work.before(at.b, m);
+  return at;
+}
+// The units of a CTA's range, one after the other.
+struct Segments {
+  const TileWork &work;
+  Place at;
+  int t0, t1, cost;
+  __device__ __forceinline__ Segments(const TileWork &w, const Place &start) : work(w), at(start) { load(); }
+  __device__ __forceinline__ void load() {
+    if (at.left <= 0) return;
+    cost = work.cost(at.b, at.m);
+    t0 = at.pos;
+    t1 = (int)min((int64_t)cost, t0 + at.left);
+  }
+  __device__ __forceinline__ bool valid() const { return at.left > 0; }
+  __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == cost; }
+  __device__ __forceinline__ int rows() const { return min(256, work.p.rows_kv - 256 * at.m); }
+  __device__ __forceinline__ ChunkView view() const { return chunk_view(work.p, at.b, 256 * at.m, rows()); }
+  __device__ __forceinline__ void next() {
+    at.left -= t1 - t0;
+    at.pos = 0;
+    if (++at.m == work.p.blocks) {
+      at.m = 0;
+      if (++at.kvh == work.p.a.kv_heads) at.kvh = 0, ++at.b;
+    }
+    load();
+  }
+};
+
+// ------------------------------------------------------------ loader of tiles
+// Lists of the next tile are read while the slots of this one are awaited.
+template <int D>
+__device__ __forceinline__ void chunk_load_tiles(const TileWork &work, ChunkShared<D> &sh, uint8_t *tiles, int lane) {
+  using Shared = ChunkShared<D>;
+  constexpr int kOperand = 128 * D * 2, kSlots = Shared::kSlots;
+  const ChunkParams &p = work.p;
+  const ChunkSpace &w = p.w;
+  int n = 0, metas = 0;
+  bool ok = true;
+  for (Segments seg(work, sh.place); seg.valid() && ok; seg.next()) {
+    const int b = seg.at.b;
+    const ChunkView view = seg.view();
+    const int4 range = __ldcg(w.ranges + (int64_t)b * p.blocks + seg.at.m);
+    const uint32_t *lists = reinterpret_cast<const uint32_t *>(w.metas + (int64_t)b * w.tiles_max);
+    const uint8_t *src = w.tiles + ((int64_t)b * p.a.kv_heads + seg.at.kvh) * w.tiles_max * 2 * kOperand;
+    if (range.z == 0) {  // no tile: the slot only carries the news
+      const int slot = n % kSlots;
+      ok = mbar_wait_bounded(smem_u32(&sh.bars.kv_empty[slot]), ((n / kSlots) & 1) ^ 1);
+      if (!ok) break;
+      if (lane == 0) {
+        sh.meta[metas % Shared::kMetas].none = 1;
+        mbar_arrive(smem_u32(&sh.bars.kv_full[slot]));
       }
-      const uint32_t page = m.page[i];
-      const int mode = (int)(page & 3), ntok = (int)(page >> 2), pos0 = kBlock * m.col[i], token0 = kBlock * i;
-      const bool check = !m.whole;
-      const uint8_t *raw = ring + sh.raw_at[rs][warp];
-      auto seen = [&](int row) { return row < ntok && view.any(pos0 + row); };
-      // a slab record's two scales share the unit behind the payload
-      auto scales = [&](int md) {
-        return reinterpret_cast<const __half *>(raw + payload_bytes(D, md)) + (SLAB ? kv : 0);
-      };
-      if (mode == AKV_MODE_INT4) {
-        if (kv) dequant_page<D, AKV_MODE_INT4, true, SLAB>(raw, scales(mode), lg, tile, token0, lane, check, seen);
-        else dequant_page<D, AKV_MODE_INT4, false, SLAB>(raw, scales(mode), lg, tile, token0, lane, check, seen);
-      } else if (mode == AKV_MODE_INT8) {
-        if (kv) dequant_page<D, AKV_MODE_INT8, true, SLAB>(raw, scales(mode), lg, tile, token0, lane, check, seen);
-        else dequant_page<D, AKV_MODE_INT8, false, SLAB>(raw, scales(mode), lg, tile, token0, lane, check, seen);
-      } else if (mode == AKV_MODE_FP16) {
-        if (kv) dequant_page<D, AKV_MODE_FP16, true, SLAB>(raw, nullptr, lg, tile, token0, lane, check, seen);
-        else dequant_page<D, AKV_MODE_FP16, false, SLAB>(raw, nullptr, lg, tile, token0, lane, check, seen);
-      } else if (kv) {  // no page: its tokens are masked, and V is finite
+      ++n, ++metas;
+      continue;
+    }
+    auto tile_at = [&](int t) { return t < range.x ? t : range.y + (t - range.x); };
+    uint32_t next = __ldcg(lists + 16ll * tile_at(seg.t0) + (lane & 15));
+    for (int t = seg.t0; t < seg.t1 && ok; ++t) {
+      const uint32_t word = next;
+      if (t + 1 < seg.t1) next = __ldcg(lists + 16ll * tile_at(t + 1) + (lane & 15));
+      const uint32_t page = __shfl_sync(0xffffffffu, word, 8 + (lane & 7));
+      const int col = (int)__shfl_sync(0xffffffffu, word, lane & 7);
+      const bool whole = __all_sync(0xffffffffu, (page & 3u) != 0 && (page >> 2) == kBlock && view.whole_page(col));
 #pragma unroll
-        for (int c = 0; c < D / 16; ++c) {
-          const int e = 256 * c + 8 * lane;
-          *reinterpret_cast<uint4 *>(tile + panel_offset(token0 + e / D, (e % D) / 8)) = make_uint4(0u, 0u, 0u, 0u);
+      for (int kv = 0; kv < 2; ++kv) {
+        const int slot = n % kSlots;
+        ok = mbar_wait_bounded(smem_u32(&sh.bars.kv_empty[slot]), ((n / kSlots) & 1) ^ 1);
+        if (!ok) break;
+        ++n;
+        if (kv == 0) {  // the slot being free, the meta's last user is past it too
+          TileMeta &m = sh.meta[metas++ % Shared::kMetas];
+          if (lane < 16) reinterpret_cast<uint32_t *>(&m)[lane] = word;
+          if (lane == 0) m.last = t + 1 == seg.t1, m.whole = whole, m.none = 0;
+          __syncwarp();
+        }
+        if (lane == 0) {
+          const uint32_t bar = smem_u32(&sh.bars.kv_full[slot]);
+          mbar_expect_tx(bar, kOperand);
+          bulk_g2s(smem_u32(tiles + slot * kOperand), src + ((int64_t)tile_at(t) * 2 + kv) * kOperand, kOperand, bar);
         }
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&sh.bars.raw_empty[rs]));
     }
-    if (dead) break;
-    const bool last = m.last;
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(smem_u32(&sh.bars.kv_full[slot]));
-    if (kv && last) break;
   }
-  if (dead && lane == 0) set_status(p.a.status, AKV_DEV_TIMEOUT);
+  if (!ok) {
+    if (lane == 0) set_status(p.a.status, AKV_DEV_TIMEOUT);
+    for (int i = max(0, n - kSlots); i < n; ++i)  // let the copies in flight land (bounded)
+      if (!mbar_wait_bounded(smem_u32(&sh.bars.kv_full[i % kSlots]), (i / kSlots) & 1)) break;
+  }
 }
 
 // ---------------------------------------------------------------- MMA issue
-// One thread issues every MMA; they execute in the order of issue, so a row
-// tile's S may overwrite the P that the MMA before it read.
-template <int D, int NT, int kSlots>
-__device__ __forceinline__ void chunk_mma(const ChunkParams &p, ChunkShared &sh, const uint8_t *q_tiles,
-                                          const uint8_t *tiles, uint32_t tmem) {
-  constexpr int kOperand = 128 * D * 2;
-  constexpr uint32_t kQk = mma_idesc(kTileTokens, false), kPv = mma_idesc(D, true);
-  const uint32_t q0 = smem_u32(q_tiles), kv0 = smem_u32(tiles);
-  ChunkBars &bar = sh.bars;
-  auto wait = [&](uint64_t &b, int phase) { return mbar_wait_bounded(smem_u32(&b), phase & 1); };
-  auto scores = [&](int x, int slot) {
+// One thread issues every MMA; they execute in the order of issue, so a stream's S
+// may overwrite the P that the MMA before it read.
+template <int D>
+struct MmaIssuer {
+  static constexpr int kOperand = 128 * D * 2, kSlots = ChunkShared<D>::kSlots;
+  static constexpr uint32_t kQk = mma_idesc(kTileTokens, false), kPv = mma_idesc(D, true);
+  ChunkBars &bar;
+  uint32_t q0, kv0, tmem;
+  int n = 0;               // fills taken, in order K0 V0 K1 V1 ...
+  int weights[2] = {0, 0}; // P tiles taken of each stream
+
+  __device__ __forceinline__ MmaIssuer(ChunkBars &b, uint32_t tm, const uint8_t *q, const uint8_t *kv)
+      : bar(b), q0(smem_u32(q)), kv0(smem_u32(kv)), tmem(tm) {}
+  __device__ __forceinline__ bool wait(uint64_t &b, int phase) const { return mbar_wait_bounded(smem_u32(&b), phase & 1); }
+  __device__ __forceinline__ bool filled(int fill) const {
+    const bool ok = wait(bar.kv_full[fill % kSlots], fill / kSlots);
+    tc_fence_after();
+    return ok;
+  }
+  __device__ __forceinline__ void release(int fill) const { tc_commit(smem_u32(&bar.kv_empty[fill % kSlots])); }
+  // Descriptors differ in the start address alone, in 16-byte units of its low word.
+  __device__ __forceinline__ static uint64_t at(uint64_t desc, uint32_t bytes) { return desc + (bytes >> 4); }
+  // S of stream x from Q tile `q` and K in `fill`.
+  __device__ __forceinline__ void scores(int x, int q, int fill) const {
+    const uint64_t qd = at(operand_desc(q0, 16, 1024), q * kOperand), kd = at(operand_desc(kv0, 16, 1024), fill % kSlots * kOperand);
 #pragma unroll
     for (int k = 0; k < D / 16; ++k) {
-      const uint32_t at = (k >> 2) * kPanel + (k & 3) * 32;
-      tc_mma_ss(tmem + kTmemS + 128 * x, operand_desc(q0 + x * kOperand + at, 16, 1024),
-                operand_desc(kv0 + slot * kOperand + at, 16, 1024), kQk, k > 0);
+      const uint32_t off = (k >> 2) * kPanel + (k & 3) * 32;
+      tc_mma_ss(tmem + kTmemS + 128 * x, at(qd, off), at(kd, off), kQk, k > 0);
     }
-  };
-  auto values = [&](int x, int slot, bool accumulate) {
-#pragma unroll
-    for (int k = 0; k < kTileTokens / 16; ++k)
-      tc_mma_ts(tmem + kTmemO + 128 * x, tmem + kTmemS + 128 * x + 8 * k,
-                operand_desc(kv0 + slot * kOperand + k * 2048, kPanel, 1024), kPv, accumulate || k > 0);
-  };
-  bool ok = wait(bar.q_full, 0) && wait(bar.kv_full[0], 0);
-  if (ok && sh.meta[0].none) {  // nothing to attend: the softmax only has to know
-    for (int x = 0; x < NT; ++x) mbar_arrive(smem_u32(&bar.s_full[x]));
-    return;
+    tc_commit(smem_u32(&bar.s_full[x]));
   }
-  if (ok) {
+  // O of stream x; P's first 64 tokens lie at S's columns 0-31, the others at 64-95.
+  __device__ __forceinline__ bool values(int x, int fill, bool accumulate) {
+    const uint64_t vd = at(operand_desc(kv0, kPanel, 1024), fill % kSlots * kOperand);
+    if (!wait(bar.p_full[x], weights[x]++)) return false;
     tc_fence_after();
 #pragma unroll
-    for (int x = 0; x < NT; ++x) {
-      scores(x, 0);
-      tc_commit(smem_u32(&bar.s_full[x]));
-    }
-    tc_commit(smem_u32(&bar.kv_empty[0]));
+    for (int k = 0; k < kTileTokens / 16; ++k)
+      tc_mma_ts(tmem + kTmemO + 128 * x, tmem + kTmemS + 128 * x + 8 * k + (k >= 4 ? 32 : 0), at(vd, k * 2048), kPv,
+                accumulate || k > 0);
+    return true;
   }
-  for (int j = 0; ok; ++j) {
-    const bool last = sh.meta[j % kMetas].last;
-    const int vn = 2 * j + 1, kn = 2 * j + 2, vs = vn % kSlots, ks = kn % kSlots;
+  __device__ __forceinline__ void outputs(int streams) const {
+    for (int x = 0; x < streams; ++x) tc_commit(smem_u32(&bar.o_full[x]));
+  }
+};
+
+// Two row tiles (one where the block has no more rows) share every tile of tokens.
+template <int D>
+__device__ __forceinline__ void chunk_mma(const TileWork &work, ChunkShared<D> &sh, const uint8_t *q_tiles,
+                                          const uint8_t *tiles) {
+  using Shared = ChunkShared<D>;
+  MmaIssuer<D> mma(sh.bars, sh.tmem, q_tiles, tiles);
+  int metas = 0, loads[2] = {0, 0};
+  bool ok = true;
+  for (Segments seg(work, sh.place); seg.valid() && ok; seg.next()) {
+    const int streams = seg.rows() > 128 ? 2 : 1;
+    ok = mma.wait(mma.bar.q_full[0], loads[0]++) && (streams == 1 || mma.wait(mma.bar.q_full[1], loads[1]++)) &&
+         mma.filled(mma.n);
+    if (!ok) break;
+    if (sh.meta[metas % Shared::kMetas].none) {  // nothing to attend: the softmax only has to know
+      mbar_arrive(smem_u32(&mma.bar.kv_empty[mma.n % Shared::kSlots]));
+      ++mma.n, ++metas;
+      for (int x = 0; x < streams; ++x) mbar_arrive(smem_u32(&mma.bar.s_full[x]));
+      mma.outputs(streams);
+      continue;
+    }
+    int k_fill = mma.n++;
+    mma.scores(0, 0, k_fill);
+    if (streams == 2) mma.scores(1, 1, k_fill);
+    mma.release(k_fill);
+    for (bool first = true;; first = false) {
+      const bool last = sh.meta[metas++ % Shared::kMetas].last;
+      const int v_fill = mma.n++;
+      if (!last) k_fill = mma.n++;
+      ok = mma.filled(v_fill);
 #pragma unroll
-    for (int x = 0; x < NT; ++x) {
-      ok = ok && wait(bar.p_full[x], j) && (x > 0 || wait(bar.kv_full[vs], vn / kSlots));
-      if (!ok) break;
-      tc_fence_after();
-      values(x, vs, j > 0);
-      if (x == NT - 1) tc_commit(smem_u32(&bar.kv_empty[vs]));
-      if (last) {
-        tc_commit(smem_u32(&bar.o_full[x]));
-        continue;
+      for (int x = 0; x < 2; ++x) {
+        if (!ok || x >= streams) break;
+        ok = mma.values(x, v_fill, !first);
+        if (x == streams - 1) mma.release(v_fill);
+        if (!ok || last) continue;
+        if (x == 0) ok = mma.filled(k_fill);
+        if (!ok) break;
+        mma.scores(x, x, k_fill);
+        if (x == streams - 1) mma.release(k_fill);
       }
-      ok = x > 0 || wait(bar.kv_full[ks], kn / kSlots);
-      if (!ok) break;
-      tc_fence_after();
-      scores(x, ks);
-      tc_commit(smem_u32(&bar.s_full[x]));
-      if (x == NT - 1) tc_commit(smem_u32(&bar.kv_empty[ks]));
+      if (!ok || last) break;
     }
-    if (last) break;
+    if (ok) mma.outputs(streams);
   }
-  if (!ok) set_status(p.a.status, AKV_DEV_TIMEOUT);
+  if (!ok) set_status(work.p.a.status, AKV_DEV_TIMEOUT);
 }
 
 // ----------------------------------------------------------------- softmax
-// Load row tile x of Q into its operand tile: a warp takes two rows of head_dim
-// 128 (four of 64) at a time, 16 bytes a lane.  A negative softmax scale is
+// Load row tile x of Q into its operand tile, 16 rows a warp: two rows of head_dim
+// 128 (four of 64) at a time, 16 bytes a lane, all of them in flight.  A negative softmax scale is
 // folded into Q's sign (exact), so that the row max is the max of the products.
 template <int D>
 __device__ __forceinline__ void load_rows(const ChunkParams &p, const ChunkView &view, int b, int kvh, int x, int warp,
@@ -514,12 +477,12 @@ __device__ __forceinline__ void load_rows(const ChunkParams &p, const ChunkView 
   const ChunkArgs &a = p.a;
   const uint32_t flip = p.q_sign < 0 ? 0x80008000u : 0u, keep = p.q_sign == 0 ? 0u : 0xffffffffu;
   const int unit = lane % kUnits;
-#pragma unroll 4
-  for (int i = 0; i < 32; i += kPer) {
-    const int row = 32 * warp + i + lane / kUnits, r = 128 * x + row;
+#pragma unroll
+  for (int i = 0; i < 16; i += kPer) {
+    const int row = 16 * warp + i + lane / kUnits, r = 128 * x + row;
     uint4 v = make_uint4(0u, 0u, 0u, 0u);
     if (r < view.n) {
-      const int rho = view.row0 + r, t = rho / p.heads_per_kv, h = kvh * p.heads_per_kv + (rho - t * p.heads_per_kv);
+      const int rho = view.row0 + r, t = fdiv(rho, p.fd_hpk), h = kvh * p.heads_per_kv + (rho - t * p.heads_per_kv);
       v = __ldg(reinterpret_cast<const uint4 *>(a.q + (int64_t)b * a.q_bs + (int64_t)h * a.q_hs + (int64_t)t * a.q_ts) + unit);
       v.x = (v.x ^ flip) & keep, v.y = (v.y ^ flip) & keep, v.z = (v.z ^ flip) & keep, v.w = (v.w ^ flip) & keep;
     }
@@ -531,224 +494,261 @@ __device__ __forceinline__ uint32_t bits_below(int n) {  // the n lowest of 16 b
   return n <= 0 ? 0u : (n >= 16 ? 0xffffu : (1u << n) - 1u);
 }
 
-template <int D>
-__device__ __forceinline__ void chunk_softmax(const ChunkParams &p, ChunkShared &sh, const ChunkView &view, int b,
-                                              int kvh, int x, int warp, int lane, uint32_t tmem) {
-  const uint32_t lane_base = (uint32_t)(32 * warp) << 16;
-  const uint32_t ts = tmem + lane_base + kTmemS + 128 * x, to = tmem + lane_base + kTmemO + 128 * x;
-  const int r = 128 * x + 32 * warp + lane;
-  const int at = view.at_first + (view.row0 + min(r, view.n - 1)) / p.heads_per_kv;
-  const float c = p.scale_log2;
-  constexpr float kNegInf = -INFINITY, kSlack = 8.f;
-  float m = kNegInf, l = 0.f;
-  bool dead = false;
-  for (int j = 0;; ++j) {
-    if (!mbar_wait_bounded(smem_u32(&sh.bars.s_full[x]), j & 1)) {
-      dead = true;
-      break;
-    }
-    tc_fence_after();
-    const TileMeta &meta = sh.meta[j % kMetas];
-    const bool last = meta.last;
-    if (meta.none) break;
-    float s[128];
+// The larger of three, NaN if one is NaN.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// Of every 16 pairs of weights, this many are worked out on the FMA pipe
+// (exp2_poly), the rest by ex2: the special-function unit takes one result a lane
+// and four clocks, and alone would take longer than the MMAs of a tile.
+constexpr int kPolyPairs = 0;
+// 2^x for two finite or -inf x <= 9: x = n + f with n whole and |f| <= 1/2 (adding
+// and taking away 1.5 * 2^23 rounds to whole numbers), 2^f by the degree-4
+// polynomial of least largest relative error on that range (2.6e-6, found with
+// Remez's exchange; the rounding to fp16 that follows is 2^-11), and n added to the
+// exponent bits.  Below 2^-126 it stays there: such a weight is 0 in fp16.
+__device__ __forceinline__ uint64_t exp2_poly(uint64_t x) {
+  auto twice = [](float v) { return f2_pack(v, v); };
+  x = f2_pack(fmaxf(f2_lo(x), -126.f), fmaxf(f2_hi(x), -126.f));
+  const uint64_t t = f2_add(x, twice(12582912.f));
+  const uint64_t f = f2_sub(x, f2_sub(t, twice(12582912.f)));
+  uint64_t p = f2_fma(twice(0.009570102207362652f), f, twice(0.05591785907745361f));
+  p = f2_fma(p, f, twice(0.240247443318367f));
+  p = f2_fma(p, f, twice(0.6931217908859253f));
+  p = f2_fma(p, f, twice(0.9999992847442627f));
+  const uint32_t lo = ((uint32_t)t << 23) + (uint32_t)p, hi = ((uint32_t)(t >> 32) << 23) + (uint32_t)(p >> 32);
+  return (uint64_t)lo | ((uint64_t)hi << 32);
+}
+
+// 32 normalised outputs of a row.
+__device__ __forceinline__ void store_out32(__half *out, const float (&o)[32], float inv, bool vector) {
+  uint32_t w[16];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) tc_ld32(ts + 32 * i, s + 32 * i);
-    tc_wait_ld();
-    if (!meta.whole) {
+  for (int k = 0; k < 16; ++k) w[k] = pack_f16x2(o[2 * k] * inv, o[2 * k + 1] * inv);
+  if (vector) {
 #pragma unroll
-      for (int g = 0; g < kTilePages; ++g) {
-        const int pos0 = kBlock * meta.col[g], ntok = (int)(meta.page[g] >> 2);
-        const uint32_t bits = bits_below(min(ntok, at - pos0 + 1)) &
-                              (~bits_below(at - view.window - pos0 + 1) | bits_below(view.sinks - pos0));
+    for (int k = 0; k < 4; ++k)
+      reinterpret_cast<uint4 *>(out)[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+  } else {
 #pragma unroll
-        for (int i = 0; i < kBlock; ++i)
-          if (!((bits >> i) & 1u)) s[kBlock * g + i] = kNegInf;
-      }
-    }
-    float tops[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) tops[i] = s[i];
-#pragma unroll
-    for (int i = 8; i < 128; ++i) tops[i % 8] = fmaxf(tops[i % 8], s[i]);
-    const float top = c * fmaxf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])),
-                                fmaxf(fmaxf(tops[4], tops[5]), fmaxf(tops[6], tops[7])));
-    // S of this tile came after O of the tile before it, so O is at rest here.
-    if (__any_sync(0xffffffffu, top > m + kSlack)) {
-      const float n = fmaxf(m, top);
-      const float w = n == kNegInf ? 1.f : ex2(m - n);
-      l *= w, m = n;
-      if (j > 0) {
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-          float o[32];
-          tc_ld32(to + 32 * i, o);
-          tc_wait_ld();
-#pragma unroll
-          for (int k = 0; k < 32; ++k) o[k] *= w;
-          tc_st32(to + 32 * i, reinterpret_cast<const uint32_t *>(o));
-        }
-      }
-    }
-    const float neg = m == kNegInf ? 0.f : -m;
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      uint32_t pk[32];
-#pragma unroll
-      for (int k = 0; k < 32; ++k) {
-        const float p0 = ex2(fmaf(s[64 * i + 2 * k], c, neg)), p1 = ex2(fmaf(s[64 * i + 2 * k + 1], c, neg));
-        sum[2 * (k & 1)] += p0, sum[2 * (k & 1) + 1] += p1;
-        pk[k] = pack_f16x2(p0, p1);
-      }
-      tc_st32(ts + 32 * i, pk);
-    }
-    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-    tc_wait_st();
-    tc_fence_before();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(smem_u32(&sh.bars.p_full[x]));
-    if (last) break;
-  }
-  const bool none = sh.meta[0].none;  // set once, for a CTA without a tile
-  if (!dead && !none && !mbar_wait_bounded(smem_u32(&sh.bars.o_full[x]), 0)) dead = true;
-  if (dead) {
-    if (lane == 0) set_status(p.a.status, AKV_DEV_TIMEOUT);
-    return;
-  }
-  tc_fence_after();
-  const ChunkArgs &a = p.a;
-  const int rho = view.row0 + r, t = rho / p.heads_per_kv, h = kvh * p.heads_per_kv + (rho - t * p.heads_per_kv);
-  __half *out = a.out + (int64_t)b * a.o_bs + (int64_t)h * a.o_hs + (int64_t)t * a.o_ts;
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i) {
-    float o[32];
-    tc_ld32(to + 32 * i, o);
-    tc_wait_ld();
-    if (r >= view.n) continue;
-    uint32_t w[16];
-#pragma unroll
-    for (int k = 0; k < 16; ++k) w[k] = pack_f16x2(l > 0.f ? o[2 * k] * inv : l, l > 0.f ? o[2 * k + 1] * inv : l);
-    if (p.vector_out) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        reinterpret_cast<uint4 *>(out + 32 * i)[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 16; ++k) {
-        out[32 * i + 2 * k] = __ushort_as_half((unsigned short)(w[k] & 0xffff));
-        out[32 * i + 2 * k + 1] = __ushort_as_half((unsigned short)(w[k] >> 16));
-      }
+    for (int k = 0; k < 16; ++k) {
+      out[2 * k] = __ushort_as_half((unsigned short)(w[k] & 0xffff));
+      out[2 * k + 1] = __ushort_as_half((unsigned short)(w[k] >> 16));
     }
   }
 }
 
+// The softmax of row tile x over one CTA's segments: 8 warps, two threads a row, one
+// for tokens 0-63 of a tile and one for 64-127 (a warp reaches the TMEM lanes of its
+// number mod 4).  They agree on the row's max through shared memory.  One thread a row
+// would leave a scheduler one warp of this row tile, which waits for its own
+// instructions most of the time.
+template <int D>
+__device__ __forceinline__ void chunk_softmax(const TileWork &work, ChunkShared<D> &sh, uint8_t *q_tile, int x, int warp,
+                                              int lane) {
+  using Shared = ChunkShared<D>;
+  constexpr int kRowStride = D + 4, kOut = D / 2;
+  constexpr float kNegInf = -INFINITY, kSlack = 8.f;
+  const ChunkParams &p = work.p;
+  const ChunkArgs &a = p.a;
+  const int quarter = warp & 3, half = warp >> 2;
+  const uint32_t base = sh.tmem + ((uint32_t)(32 * quarter) << 16);
+  const uint32_t ts = base + kTmemS + 128 * x + 64 * half, to = base + kTmemO + 128 * x + kOut * half;
+  const float c = p.scale_log2;
+  const int tile_row = 32 * quarter + lane, r = 128 * x + tile_row;  // row of the tile, of the block
+  const int pair = 1 + 4 * x + quarter;                              // the named barrier of the row's two warps
+  float *mine = &sh.shared_rows[x][half][tile_row], *theirs = &sh.shared_rows[x][half ^ 1][tile_row];
+  // The partner read the last value before the scores that this one is about came.
+  auto exchange = [&](float v) {
+    *mine = v;
+    asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
+    return *theirs;
+  };
+  int tiles = 0, metas = 0, segments = 0;
+  int4 cut = make_int4(0, 0, 0, 0);
+  bool ok = true;
+  for (Segments seg(work, sh.place); seg.valid() && ok; seg.next()) {
+    const ChunkView view = seg.view();
+    const int b = seg.at.b, kvh = seg.at.kvh;
+    if (seg.t0 > 0) cut.x = seg.t1 == seg.cost ? 2 : 1;
+    else if (seg.t1 < seg.cost) cut.y = b, cut.z = kvh, cut.w = seg.at.m + 1;
+    if (128 * x >= view.n) {  // the block has one row tile: its tiles are only counted
+      const int4 range = __ldcg(p.w.ranges + (int64_t)b * p.blocks + seg.at.m);
+      metas += range.z == 0 ? 1 : seg.t1 - seg.t0;
+      continue;
+    }
+    load_rows<D>(p, view, b, kvh, x, warp, lane, q_tile);
+    fence_proxy_async_smem();
+    tc_fence_before();  // the reads of the last segment's O come before this segment's MMAs
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&sh.bars.q_full[x]));
+    const bool active = r - lane < view.n;  // a warp without rows only keeps the barriers going
+    const int at = view.at_first + fdiv(view.row0 + min(r, view.n - 1), p.fd_hpk);
+    float m = kNegInf, l = 0.f;
+    bool first = true;
+    while (true) {
+      ok = mbar_wait_bounded(smem_u32(&sh.bars.s_full[x]), tiles & 1);
+      if (!ok) break;
+      ++tiles;
+      tc_fence_after();
+      const TileMeta &meta = sh.meta[metas++ % Shared::kMetas];
+      if (meta.none) break;
+      const bool last = meta.last;
+      if (active) {
+        float s[64];
+        tc_ld32(ts, s);
+        tc_ld32(ts + 32, s + 32);
+        tc_wait_ld();
+        if (!meta.whole) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int pos0 = kBlock * meta.col[4 * half + g], ntok = (int)(meta.page[4 * half + g] >> 2);
+            const uint32_t bits = bits_below(min(ntok, at - pos0 + 1)) &
+                                  (~bits_below(at - view.window - pos0 + 1) | bits_below(view.sinks - pos0));
+#pragma unroll
+            for (int i = 0; i < kBlock; ++i)
+              if (!((bits >> i) & 1u)) s[kBlock * g + i] = kNegInf;
+          }
+        }
+        float tops[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int i = 4; i < 60; i += 8)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) tops[k] = max3(tops[k], s[i + k], s[i + 4 + k]);
+        float top = max3(max3(tops[0], tops[1], s[60]), max3(tops[2], tops[3], s[61]), max3(s[62], s[63], s[63]));
+        top = c * max3(top, exchange(top), top);
+        // S of this tile came after O of the row tile's tile before it, so O is at rest
+        // here.  A NaN score makes the row's max, and with it the row, NaN.
+        if (__any_sync(0xffffffffu, !(top <= m + kSlack))) {
+          const float n = max3(m, top, top);
+          const float w = n == kNegInf ? 1.f : ex2(m - n);
+          l *= w, m = n;
+          if (!first) {
+#pragma unroll 1
+            for (int i = 0; i < kOut / 16; ++i) {
+              float o[16];
+              tc_ld16(to + 16 * i, o);
+              tc_wait_ld();
+#pragma unroll
+              for (int k = 0; k < 16; ++k) o[k] *= w;
+              tc_st16(to + 16 * i, reinterpret_cast<const uint32_t *>(o));
+            }
+          }
+        }
+        const float neg = m == kNegInf ? 0.f : -m;
+        const uint64_t c2 = f2_pack(c, c), neg2 = f2_pack(neg, neg);
+        uint64_t sum[2] = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // 16 tokens at a time; P replaces the thread's own scores
+          uint32_t pk[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const uint64_t x2 = f2_fma(f2_pack(s[16 * i + 2 * k], s[16 * i + 2 * k + 1]), c2, neg2);
+            const uint64_t p2 = k < kPolyPairs ? exp2_poly(x2) : f2_pack(ex2(f2_lo(x2)), ex2(f2_hi(x2)));
+            sum[k & 1] = f2_add(sum[k & 1], p2);
+            pk[k] = pack_f16x2(f2_lo(p2), f2_hi(p2));
+          }
+          tc_st8(ts + 8 * i, pk);
+        }
+        const uint64_t both = f2_add(sum[0], sum[1]);
+        l += f2_lo(both) + f2_hi(both);
+        tc_wait_st();
+        tc_fence_before();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sh.bars.p_full[x]));
+      first = false;
+      if (last) break;
+    }
+    ok = ok && mbar_wait_bounded(smem_u32(&sh.bars.o_full[x]), segments++ & 1);
+    if (!ok) break;
+    tc_fence_after();
+    if (!active) continue;
+    l += exchange(l);
+    // The block's rows, or this range's share of them.
+    const bool direct = seg.whole();
+    float *part = p.partials + ((2ll * blockIdx.x + (seg.t0 > 0 ? 0 : 1)) * 256 + r) * kRowStride;
+    const int rho = view.row0 + r, tok = fdiv(rho, p.fd_hpk), h = kvh * p.heads_per_kv + (rho - tok * p.heads_per_kv);
+    __half *out = a.out + (int64_t)b * a.o_bs + (int64_t)h * a.o_hs + (int64_t)tok * a.o_ts + kOut * half;
+    const float inv = l > 0.f ? 1.f / l : l;  // a row that saw nothing is 0, a NaN stays one
+#pragma unroll
+    for (int i = 0; i < kOut / 32; ++i) {
+      float o[32];
+      tc_ld32(to + 32 * i, o);
+      tc_wait_ld();
+      if (first) {  // O was never written
+#pragma unroll
+        for (int k = 0; k < 32; ++k) o[k] = 0.f;
+      }
+      if (r >= view.n) continue;
+      if (direct) {
+        store_out32(out + 32 * i, o, inv, p.vector_out);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          reinterpret_cast<float4 *>(part + kOut * half + 32 * i)[k] =
+              make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+      }
+    }
+    if (!direct && half == 0 && r < view.n) *reinterpret_cast<float2 *>(part + D) = make_float2(m, l);
+  }
+  if (x == 0 && warp == 0 && lane == 0) p.w.cuts[blockIdx.x] = cut;
+  if (!ok) {  // release a partner that may be waiting for this warp
+    asm volatile("bar.arrive %0, 64;" ::"r"(pair) : "memory");
+    if (lane == 0) set_status(a.status, AKV_DEV_TIMEOUT);
+  }
+}
+
 // ---------------------------------------------------------- CTA set-up
-__device__ __forceinline__ void chunk_begin(ChunkShared &sh, int nt, int kv_arrivals, int alloc_warp) {
+template <int D>
+__device__ __forceinline__ void chunk_begin(const TileWork &work, ChunkShared<D> &sh, int alloc_warp) {
   if (threadIdx.x == 0) {
     ChunkBars &bar = sh.bars;
-    for (int i = 0; i < kItems; ++i) mbar_init(smem_u32(&bar.raw_full[i]), 1), mbar_init(smem_u32(&bar.raw_empty[i]), 4);
-    for (int i = 0; i < kMaxSlots; ++i)
-      mbar_init(smem_u32(&bar.kv_full[i]), kv_arrivals), mbar_init(smem_u32(&bar.kv_empty[i]), 1);
-    mbar_init(smem_u32(&bar.q_full), 4 * nt);
+    for (int i = 0; i < kMaxSlots; ++i) mbar_init(smem_u32(&bar.kv_full[i]), 1), mbar_init(smem_u32(&bar.kv_empty[i]), 1);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&bar.q_full[i]), 8);
       mbar_init(smem_u32(&bar.s_full[i]), 1);
-      mbar_init(smem_u32(&bar.p_full[i]), 4);
+      mbar_init(smem_u32(&bar.p_full[i]), 8);
       mbar_init(smem_u32(&bar.o_full[i]), 1);
     }
     fence_mbar_init();
-    sh.meta[0].none = 0;
   }
   if ((int)(threadIdx.x >> 5) == alloc_warp) {
     tmem_alloc(smem_u32(&sh.tmem), kTmemCols);
     tmem_release_permit();
   }
+  grid_dependency_wait();
+  allow_dependents_launch();
+  if (threadIdx.x < 32) {
+    const Place at = find_place(work, blockIdx.x);
+    if (threadIdx.x == 0) sh.place = at;
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
 }
-__device__ __forceinline__ void chunk_end(uint32_t tmem, int alloc_warp) {
+template <int D>
+__device__ __forceinline__ void chunk_end(ChunkShared<D> &sh, int alloc_warp) {
   tc_fence_before();
   __syncthreads();
   if ((int)(threadIdx.x >> 5) == alloc_warp) {
     tc_fence_after();
-    tmem_dealloc(tmem, kTmemCols);
+    tmem_dealloc(sh.tmem, kTmemCols);
   }
 }
-template <int D>
-__device__ __forceinline__ void chunk_rows_role(const ChunkParams &p, ChunkShared &sh, const ChunkView &view, int b,
-                                                int kvh, int x, int w, int lane, uint8_t *q_tile, uint32_t tmem) {
-  load_rows<D>(p, view, b, kvh, x, w, lane, q_tile);
-  fence_proxy_async_smem();
-  __syncwarp();
-  if (lane == 0) mbar_arrive(smem_u32(&sh.bars.q_full));
-  chunk_softmax<D>(p, sh, view, b, kvh, x, w, lane, tmem);
-}
 
-// ============================================== pages dequantised in the kernel
-constexpr int kPageSlots = 4;
-// Registers a thread: at launch, and after the split (softmax, dequantisation, loader and MMA warpgroups).
-constexpr int kPageThreads = 512;
-constexpr int kPageRegs = 128, kSoftmaxRegs = 192, kDequantRegs = 80, kIssueRegs = 48;
-static_assert(2 * kSoftmaxRegs + kDequantRegs + kIssueRegs <= 4 * kPageRegs, "a warpgroup would wait for registers");
-
-template <int D, bool SLAB, int NT>
-__global__ void __launch_bounds__(kPageThreads, 1) chunk_pages_kernel(const __grid_constant__ ChunkParams p) {
-  constexpr int kOperand = 128 * D * 2;
-  extern __shared__ __align__(1024) uint8_t smem[];
-  uint8_t *q_tiles = smem, *tiles = smem + NT * kOperand, *ring = tiles + kPageSlots * kOperand;
-  ChunkShared &sh = *reinterpret_cast<ChunkShared *>(ring + kRawRing);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  chunk_begin(sh, NT, 4, 13);
-  const uint32_t tmem = sh.tmem;
-  grid_dependency_wait();
-  allow_dependents_launch();
-  const int kvh = blockIdx.y, b = blockIdx.z;
-  const int row0 = (int)blockIdx.x * (128 * NT);
-  const ChunkView view = chunk_view(p, b, row0, min(128 * NT, p.rows_kv - row0));
-  if (warp < 8) {
-    const int x = warp >> 2, w = warp & 3;
-    set_registers_up<kSoftmaxRegs>();
-    if (x < NT) chunk_rows_role<D>(p, sh, view, b, kvh, x, w, lane, q_tiles + x * kOperand, tmem);
-  } else if (warp < 12) {
-    set_registers_down<kDequantRegs>();
-    chunk_dequant<D, SLAB>(p, sh, ring, tiles, view, warp - 8, lane);
-  } else {
-    set_registers_down<kIssueRegs>();
-    if (warp == 12) chunk_load<D>(p, sh, ring, view, b, kvh, lane);
-    if (warp == 13 && lane == 0) chunk_mma<D, NT, kPageSlots>(p, sh, q_tiles, tiles, tmem);
-    __syncwarp();
-  }
-  chunk_end(tmem, 13);
-}
-
-// ==================================================== pages dequantised before
-// Where many row tiles share the pages, each page is dequantised once per call
-// into operand tiles in the workspace (plan, then unpack), and the attention
-// kernel copies whole tiles:
-//   counts [batch]                resident pages the call's rows may see
-//   lists  [batch][tiles * 8]     their descriptors, in order
-//   metas  [batch][tiles]         their columns and valid tokens
-//   tiles  [batch][kv head][tile] K tile, V tile
-struct __align__(16) PageList {  // of one tile, as the kernels read it: 64 bytes
-  int32_t col[kTilePages];
-  uint32_t page[kTilePages];
-};
-struct ChunkSpace {
-  int32_t *counts;
-  int64_t *lists;
-  PageList *metas;
-  uint8_t *tiles;
-  int32_t tiles_max;
-};
-
-// One CTA per sequence: the resident pages in column order.
-__global__ void __launch_bounds__(1024) chunk_plan_kernel(const __grid_constant__ ChunkParams p, const ChunkSpace w) {
-  __shared__ int warps[32];
+// ------------------------------------------------------------ plan and unpack
+// One CTA per sequence: the resident pages in column order, and the tiles that each
+// block of 256 rows sees of them.
+__global__ void __launch_bounds__(1024) chunk_plan_kernel(const __grid_constant__ ChunkParams p) {
+  constexpr int kNear = 8192;  // columns kept for the searches below (2^17 tokens)
+  __shared__ int warps[32], near[kNear];
   grid_dependency_wait();
   allow_dependents_launch();
   const ChunkArgs &a = p.a;
+  const ChunkSpace &w = p.w;
   const int b = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const ChunkView view = chunk_view(p, b, 0, p.rows_kv);
   const int64_t *table = a.table + (int64_t)b * a.table_stride;
@@ -781,6 +781,7 @@ __global__ void __launch_bounds__(1024) chunk_plan_kernel(const __grid_constant_
     if (ok) {
       const int rank = n + before + __popc(mask & ((1u << lane) - 1u));
       list[rank] = d;
+      if (rank < kNear) near[rank] = col;
       metas[rank / kTilePages].col[rank % kTilePages] = col;
       metas[rank / kTilePages].page[rank % kTilePages] = (uint32_t)mode | ((uint32_t)desc_ntok(d) << 2);
     }
@@ -792,16 +793,61 @@ __global__ void __launch_bounds__(1024) chunk_plan_kernel(const __grid_constant_
     metas[rank / kTilePages].col[threadIdx.x] = 0, metas[rank / kTilePages].page[threadIdx.x] = 0;
   }
   if (threadIdx.x == 0) w.counts[b] = n;
+  __syncthreads();
+  // Pages of the list below a column.
+  auto below = [&](int column) {
+    int lo = 0, hi = n;
+    while (lo < hi) {
+      const int mid = (lo + hi) / 2;
+      if ((mid < kNear ? near[mid] : metas[mid / kTilePages].col[mid % kTilePages]) < column) lo = mid + 1;
+      else hi = mid;
+    }
+    return lo;
+  };
+  int4 *ranges = w.ranges + (int64_t)b * p.blocks;
+  int *prefix = w.prefix + (int64_t)b * (p.blocks + 1);
+  int sum = 0;
+  for (int base = 0; base < p.blocks; base += 1024) {
+    const int m = base + (int)threadIdx.x;
+    int cost = 0;
+    if (m < p.blocks) {
+      const ChunkView v = chunk_view(p, b, 256 * m, min(256, p.rows_kv - 256 * m));
+      const int end = v.at_hi < 0 ? 0 : (below(v.at_hi / kBlock + 1) + kTilePages - 1) / kTilePages;
+      const int sinks = min(end, (below(v.lead) + kTilePages - 1) / kTilePages);
+      const int first = max(sinks, min(end, below(v.first) / kTilePages));
+      const int tiles = sinks + (end - first);
+      ranges[m] = make_int4(sinks, first, tiles, 0);
+      cost = max(1, tiles);
+    }
+    int upto = cost;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += o;
+    }
+    if (lane == 31) warps[warp] = upto;
+    __syncthreads();
+    int before = 0, all = 0;
+    for (int i = 0; i < 32; ++i) {
+      if (i == warp) before = all;
+      all += warps[i];
+    }
+    __syncthreads();
+    if (m < p.blocks) prefix[m] = sum + before + upto - cost;
+    sum += all;
+  }
+  if (threadIdx.x == 0) prefix[p.blocks] = sum;
 }
 
 // One warp per (KV head, page, K or V) of a tile: 8 elements a lane and step, all
 // loads of a page issued before the first is converted.
 template <int D, bool SLAB>
-__global__ void __launch_bounds__(256) chunk_unpack_kernel(const __grid_constant__ ChunkParams p, const ChunkSpace w) {
+__global__ void __launch_bounds__(256) chunk_unpack_kernel(const __grid_constant__ ChunkParams p) {
   constexpr int kOperand = 128 * D * 2, NC = D / 16, kUnits = D / 8, kRows = 32 / kUnits;
   grid_dependency_wait();
   allow_dependents_launch();
   const ChunkArgs &a = p.a;
+  const ChunkSpace &w = p.w;
   const int tile = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 31;
   if (tile * kTilePages >= __ldcg(w.counts + b)) return;
   const ChunkView view = chunk_view(p, b, 0, p.rows_kv);
@@ -838,136 +884,102 @@ __global__ void __launch_bounds__(256) chunk_unpack_kernel(const __grid_constant
   }
 }
 
-// The loader of whole tiles: 32 tiles' lists at a time, one per lane, a window
-// ahead; tiles that no row of the CTA sees are passed over.
-template <int D, int kSlots>
-__device__ __forceinline__ void chunk_load_tiles(const ChunkParams &p, const ChunkSpace &w, ChunkShared &sh,
-                                                 uint8_t *tiles, const ChunkView &view, int b, int kvh, int lane) {
+// Warps 0-15 softmax, 16 loader, 17 MMA issue (18 and 19 make up the warpgroup).
+// Registers a thread: at launch, and after the split.
+constexpr int kTileThreads = 640;
+constexpr int kTileRegs = 96, kSoftmaxRegs = 104, kIssueRegs = 64;
+static_assert(4 * kSoftmaxRegs + kIssueRegs <= 5 * kTileRegs, "a warpgroup would wait for registers");
+
+template <int D>
+__global__ void __launch_bounds__(kTileThreads, 1) chunk_tiles_kernel(const __grid_constant__ ChunkParams p) {
   constexpr int kOperand = 128 * D * 2;
-  const int pages = __ldcg(w.counts + b), count = (pages + kTilePages - 1) / kTilePages;
-  const PageList *metas = w.metas + (int64_t)b * w.tiles_max;
-  const uint8_t *src = w.tiles + ((int64_t)b * p.a.kv_heads + kvh) * w.tiles_max * 2 * kOperand;
-  uint4 next[4], cur[4];
-  auto fetch = [&](int w0) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) next[i] = make_uint4(0u, 0u, 0u, 0u);
-    if (w0 + lane < count) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) next[i] = __ldcg(reinterpret_cast<const uint4 *>(metas + w0 + lane) + i);
-    }
-  };
-  uint32_t mask = 0, wholes = 0;
-  int win0 = 0;
-  auto prepare = [&]() {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) cur[i] = next[i];
-    const uint32_t c[8] = {cur[0].x, cur[0].y, cur[0].z, cur[0].w, cur[1].x, cur[1].y, cur[1].z, cur[1].w};
-    const uint32_t g[8] = {cur[2].x, cur[2].y, cur[2].z, cur[2].w, cur[3].x, cur[3].y, cur[3].z, cur[3].w};
-    bool some = false, whole = true;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int col = (int)c[i], p0 = kBlock * col;
-      const bool here = (g[i] & 3u) != 0;
-      some |= here && p0 <= view.at_hi && (p0 + kBlock - 1 > view.at_lo - view.window || p0 < view.sinks);
-      whole &= here && (g[i] >> 2) == kBlock && view.whole_page(col);
-    }
-    mask = __ballot_sync(0xffffffffu, some);
-    wholes = __ballot_sync(0xffffffffu, whole);
-  };
-  fetch(0);
-  prepare();
-  fetch(32);
-  auto seek = [&]() {  // to the next window with a visible tile
-    while (mask == 0 && win0 + 32 < count) {
-      win0 += 32;
-      prepare();
-      fetch(win0 + 32);
-    }
-  };
-  seek();
-  if (mask == 0) {
-    if (lane == 0) {
-      sh.meta[0].last = 1, sh.meta[0].none = 1;
-      mbar_arrive(smem_u32(&sh.bars.kv_full[0]));
-    }
-    return;
-  }
-  for (int t = 0, n = 0;; ++t) {
-    const int k = __ffs(mask) - 1, tile = win0 + k;
-    TileMeta &m = sh.meta[t % kMetas];
-    // The first of this tile's slots is free only after the tile that last used
-    // its meta has been attended, so the wait comes before the writes.
-    const int slot = n % kSlots;
-    if (!mbar_wait_bounded(smem_u32(&sh.bars.kv_empty[slot]), ((n / kSlots) & 1) ^ 1)) break;
-    if (lane == k) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) reinterpret_cast<uint4 *>(&m)[i] = cur[i];
-      m.whole = (wholes >> k) & 1u;
-    }
-    mask &= mask - 1u;
-    seek();
-    const bool last = mask == 0;
-    if (lane == 0) m.last = last, m.none = 0;
-    __syncwarp();
-    bool ok = true;
-#pragma unroll
-    for (int kv = 0; kv < 2; ++kv, ++n) {
-      const int s = n % kSlots;
-      if (kv == 1) ok = mbar_wait_bounded(smem_u32(&sh.bars.kv_empty[s]), ((n / kSlots) & 1) ^ 1);
-      if (!ok) break;
-      if (lane == 0) {
-        const uint32_t bar = smem_u32(&sh.bars.kv_full[s]);
-        mbar_expect_tx(bar, kOperand);
-        bulk_g2s(smem_u32(tiles + s * kOperand), src + ((int64_t)tile * 2 + kv) * kOperand, kOperand, bar);
-      }
-    }
-    if (!ok) {  // the copies in flight end before the CTA does: its K tile's, at most
-      mbar_wait_bounded(smem_u32(&sh.bars.kv_full[slot]), ((n - 1) / kSlots) & 1);
-      break;
-    }
-    if (last) return;
-  }
-  if (lane == 0) set_status(p.a.status, AKV_DEV_TIMEOUT);
-}
-
-constexpr int kTileThreads = 384;
-// At launch, and after the split (softmax warpgroups; loader and MMA warpgroup).
-constexpr int kTileRegs = 168, kTileSoftmaxRegs = 216, kTileIssueRegs = 72;
-static_assert(2 * kTileSoftmaxRegs + kTileIssueRegs <= 3 * kTileRegs, "a warpgroup would wait for registers");
-template <int D>
-constexpr int tile_slots() {
-  return D == 128 ? 5 : 8;
-}
-
-template <int D>
-__global__ void __launch_bounds__(kTileThreads, 1)
-    chunk_tiles_kernel(const __grid_constant__ ChunkParams p, const ChunkSpace w) {
-  constexpr int kOperand = 128 * D * 2, kSlots = tile_slots<D>();
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t *q_tiles = smem, *tiles = smem + 2 * kOperand;
-  ChunkShared &sh = *reinterpret_cast<ChunkShared *>(tiles + kSlots * kOperand);
+  ChunkShared<D> &sh = *reinterpret_cast<ChunkShared<D> *>(tiles + ChunkShared<D>::kSlots * kOperand);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  chunk_begin(sh, 2, 1, 9);
-  const uint32_t tmem = sh.tmem;
-  grid_dependency_wait();
-  allow_dependents_launch();
-  const int kvh = blockIdx.y, b = blockIdx.z;
-  const int row0 = (int)blockIdx.x * 256;
-  const ChunkView view = chunk_view(p, b, row0, min(256, p.rows_kv - row0));
-  if (warp < 8) {
-    set_registers_up<kTileSoftmaxRegs>();
-    const int x = warp >> 2;
-    chunk_rows_role<D>(p, sh, view, b, kvh, x, warp & 3, lane, q_tiles + x * kOperand, tmem);
+  const TileWork work{p};
+  chunk_begin(work, sh, 17);
+  if (warp < 16) {
+    set_registers_up<kSoftmaxRegs>();
+    const int x = warp >> 3;
+    chunk_softmax<D>(work, sh, q_tiles + x * kOperand, x, warp & 7, lane);
   } else {
-    set_registers_down<kTileIssueRegs>();
-    if (warp == 8) chunk_load_tiles<D, kSlots>(p, w, sh, tiles, view, b, kvh, lane);
-    if (warp == 9 && lane == 0) chunk_mma<D, 2, kSlots>(p, sh, q_tiles, tiles, tmem);
+    set_registers_down<kIssueRegs>();
+    if (warp == 16) chunk_load_tiles<D>(work, sh, tiles, lane);
+    if (warp == 17 && lane == 0) chunk_mma<D>(work, sh, q_tiles, tiles);
     __syncwarp();
   }
-  chunk_end(tmem, 9);
+  chunk_end(sh, 17);
 }
 
+// ------------------------------------------------------------------- merge
+// Join the partial (O, m, l) rows of the units that the ranges cut, a warp per row; a
+// share that saw nothing (m = -inf) weighs 0.  CTA c's entry of `cuts`: y, z, w - 1 the
+// unit (sequence, KV head, row block) that its range begins and does not end (w 0:
+// none); x: it goes on with a unit begun before (1), and ends it (2).  Block c joins
+// the unit that range c begins.
+template <int D>
+__global__ void __launch_bounds__(256) chunk_merge_kernel(const __grid_constant__ ChunkParams p) {
+  constexpr int VEC = D / 32, kRowStride = D + 4;
+  grid_dependency_wait();
+  allow_dependents_launch();
+  const ChunkArgs &a = p.a;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c0 = blockIdx.x;
+  const int4 cut = __ldcg(p.w.cuts + c0);
+  const int b = cut.y, kvh = cut.z, row0 = 256 * (cut.w - 1), r = blockIdx.y * 8 + warp;
+  if (cut.w == 0 || r >= p.rows_kv - row0) return;
+  int c1 = c0 + 1;
+  while (c1 < p.ctas - 1 && __ldcg(&p.w.cuts[c1].x) == 1) ++c1;
+  {
+    float m = -INFINITY, l = 0.f, acc[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
+    constexpr int CB = 4;  // shares whose loads are in flight together
+    for (int c = c0; c <= c1; c += CB) {
+      float2 ml[CB];
+      float o[CB][VEC];
+#pragma unroll
+      for (int j = 0; j < CB; ++j) {
+        ml[j].x = -INFINITY;
+        if (c + j <= c1) {
+          const float *part = p.partials + ((2ll * (c + j) + (c + j == c0 ? 1 : 0)) * 256 + r) * kRowStride;
+          ml[j] = __ldcg(reinterpret_cast<const float2 *>(part + D));
+#pragma unroll
+          for (int i = 0; i < VEC; i += 2) {
+            const float2 v = __ldcg(reinterpret_cast<const float2 *>(part + VEC * lane + i));
+            o[j][i] = v.x, o[j][i + 1] = v.y;
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < CB; ++j) {
+        if (ml[j].x == -INFINITY) continue;
+        const float top = fmaxf(m, ml[j].x), x = ex2(m - top), y = ex2(ml[j].x - top);
+        l = l * x + ml[j].y * y;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[i] = acc[i] * x + o[j][i] * y;
+        m = isnan(ml[j].x) ? ml[j].x : top;
+      }
+    }
+    const int rho = row0 + r, tok = fdiv(rho, p.fd_hpk), h = kvh * p.heads_per_kv + (rho - tok * p.heads_per_kv);
+    __half *out = a.out + (int64_t)b * a.o_bs + (int64_t)h * a.o_hs + (int64_t)tok * a.o_ts + VEC * lane;
+    const float inv = l > 0.f ? 1.f / l : l;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) out[i] = __float2half_rn(acc[i] * inv);
+  }
+}
 // ------------------------------------------------------------------- host
+// SMs of the current device (one CTA each), 0 on error.
+static int device_sms() {
+  static std::atomic<int> cached[256];
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  if (dev < 256 && (sms = cached[dev].load(std::memory_order_relaxed)) > 0) return sms;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  if (dev < 256) cached[dev].store(sms, std::memory_order_relaxed);
+  return sms;
+}
+
 // Raise a kernel's shared-memory limit, once per device, and check that it starts
 // with the registers its warpgroups then share out.
 template <typename Kernel>
@@ -983,76 +995,106 @@ static cudaError_t chunk_ready(Kernel kernel, int smem, int regs, std::atomic<bo
   return cudaSuccess;
 }
 
-template <int D, bool SLAB, int NT>
-static cudaError_t launch_pages(const ChunkParams &p) {
-  constexpr int smem = (NT + kPageSlots) * 128 * D * 2 + kRawRing + (int)sizeof(ChunkShared);
-  static_assert(smem <= 232448, "one CTA's shared memory");
-  static std::atomic<bool> ready[256];
-  if (cudaError_t err = chunk_ready(chunk_pages_kernel<D, SLAB, NT>, smem, kPageRegs, ready)) return err;
-  const dim3 grid((p.rows_kv + 128 * NT - 1) / (128 * NT), p.a.kv_heads, p.a.batch);
-  return launch_dependent(chunk_pages_kernel<D, SLAB, NT>, grid, kPageThreads, smem, p.a.stream, p);
-}
-
 template <int D, bool SLAB>
-static cudaError_t launch_tiles(const ChunkParams &p, const ChunkSpace &w) {
-  constexpr int smem = (2 + tile_slots<D>()) * 128 * D * 2 + (int)sizeof(ChunkShared);
+static cudaError_t launch_tiles(const ChunkParams &p) {
+  constexpr int smem = (2 + ChunkShared<D>::kSlots) * 128 * D * 2 + (int)sizeof(ChunkShared<D>);
   static_assert(smem <= 232448, "one CTA's shared memory");
   static std::atomic<bool> ready[256];
   if (cudaError_t err = chunk_ready(chunk_tiles_kernel<D>, smem, kTileRegs, ready)) return err;
   cudaStream_t s = p.a.stream;
-  if (cudaError_t err = launch_dependent(chunk_plan_kernel, p.a.batch, 1024, 0, s, p, w)) return err;
-  if (w.tiles_max > 0)
-    if (cudaError_t err = launch_dependent(chunk_unpack_kernel<D, SLAB>, dim3(w.tiles_max, p.a.batch, 2), 256, 0, s, p, w))
+  if (cudaError_t err = launch_dependent(chunk_plan_kernel, p.a.batch, 1024, 0, s, p)) return err;
+  // 16 KV-head-pages a warp where there are tiles enough for the device, down to one
+  const int64_t tiles = (int64_t)p.w.tiles_max * p.a.batch;
+  const int jobs = 2 * kTilePages * p.a.kv_heads / 8;  // of a tile, per warp of a CTA
+  const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(jobs, std::max<int64_t>(jobs / 16, 8 * p.ctas / std::max<int64_t>(tiles, 1))));
+  if (p.w.tiles_max > 0)
+    if (cudaError_t err =
+            launch_dependent(chunk_unpack_kernel<D, SLAB>, dim3(p.w.tiles_max, p.a.batch, parts), 256, 0, s, p))
       return err;
-  const dim3 grid((p.rows_kv + 255) / 256, p.a.kv_heads, p.a.batch);
-  return launch_dependent(chunk_tiles_kernel<D>, grid, kTileThreads, smem, s, p, w);
+  if (cudaError_t err = launch_dependent(chunk_tiles_kernel<D>, p.ctas, kTileThreads, smem, s, p)) return err;
+  return launch_dependent(chunk_merge_kernel<D>, dim3(p.ctas, std::min(32, (p.rows_kv + 7) / 8)), 256, 0, s, p);
 }
 
-// Tiles the rows of a call may see, at most.
-static int64_t space_tiles(const ChunkArgs &a) {
-  int64_t columns = a.columns;
-  if (a.window < (1 << 30)) columns = std::min<int64_t>(columns, a.lead + ((int64_t)a.window + a.rows + 2 * kBlock - 3) / kBlock);
-  return (columns + kTilePages - 1) / kTilePages;
-}
 static int64_t align256(int64_t n) { return (n + 255) & ~(int64_t)255; }
-static int64_t space_layout(const ChunkArgs &a, int64_t tiles, uint8_t *base, ChunkSpace *w) {
-  const int64_t counts = 0, lists = align256(4ll * a.batch);
-  const int64_t metas = lists + align256(8ll * kTilePages * tiles * a.batch);
-  const int64_t data = (metas + align256((int64_t)sizeof(PageList) * tiles * a.batch) + 1023) & ~(int64_t)1023;
-  if (w) {
-    w->counts = (int32_t *)(base + counts), w->lists = (int64_t *)(base + lists);
-    w->metas = (PageList *)(base + metas), w->tiles = base + data, w->tiles_max = (int32_t)tiles;
-  }
-  return data + tiles * a.batch * a.kv_heads * 2 * 128 * a.head_dim * 2;
+// The workspace of a call, and where its parts lie (p: nullable).
+static int64_t chunk_layout(const ChunkArgs &a, int sms, uint8_t *base, ChunkParams *p) {
+  const int hpk = a.q_heads / a.kv_heads;
+  const int64_t rows_kv = (int64_t)a.rows * hpk, pairs = (int64_t)a.batch * a.kv_heads;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t here = at;
+    at += align256(bytes);
+    return base + here;
+  };
+  const int64_t blocks = (rows_kv + 255) / 256;
+  int64_t columns = a.columns;  // that some row may see
+  if (a.window < (1 << 30))
+    columns = std::min<int64_t>(columns, a.lead + ((int64_t)a.window + a.rows + 2 * kBlock - 3) / kBlock);
+  const int64_t tiles = (columns + kTilePages - 1) / kTilePages;
+  ChunkSpace w;
+  w.counts = (int32_t *)take(4ll * a.batch);
+  w.lists = (int64_t *)take(8ll * kTilePages * tiles * a.batch);
+  w.metas = (PageList *)take((int64_t)sizeof(PageList) * tiles * a.batch);
+  w.ranges = (int4 *)take(16ll * blocks * a.batch);
+  w.prefix = (int32_t *)take(4ll * (blocks + 1) * a.batch);
+  w.cuts = (int4 *)take(16ll * sms);
+  float *parts = (float *)take(2ll * sms * 256 * (a.head_dim + 4) * 4);
+  w.tiles = take(tiles * pairs * 2 * 128 * a.head_dim * 2);
+  w.tiles_max = (int32_t)tiles;
+  if (p) p->w = w, p->partials = parts, p->blocks = (int32_t)blocks;
+  return at;
+}
+
+// Operand tiles are four times the bytes of INT4 pages and more, so a large batch goes
+// in slices of whole sequences that share a workspace of about this size.
+constexpr int64_t kSpaceBytes = 2ll << 30;
+static ChunkArgs slice_of(ChunkArgs a, int first, int count) {
+  a.table += first * a.table_stride;
+  if (a.seq_blocks) a.seq_blocks += first;
+  if (a.tokens) a.tokens += first;
+  a.q += first * a.q_bs, a.out += first * a.o_bs;
+  a.batch = count;
+  return a;
+}
+static int slice_batch(const ChunkArgs &a, int sms) {
+  ChunkArgs one = a;
+  one.batch = 1;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(a.batch, kSpaceBytes / chunk_layout(one, sms, nullptr, nullptr)));
 }
 
 int64_t chunk_tiles_bytes(const ChunkArgs &a) {
-  return a.rows * (a.q_heads / a.kv_heads) > 128 ? space_layout(a, space_tiles(a), nullptr, nullptr) : 0;
+  const int sms = device_sms();
+  if (sms <= 0) return -1;
+  ChunkArgs part = a;
+  part.batch = slice_batch(a, sms);
+  return chunk_layout(part, sms, nullptr, nullptr);
 }
 
-int chunk_tiles_launch(const ChunkArgs &a, void *workspace, int64_t workspace_bytes) {
-  ChunkParams p;
-  p.a = a;
-  p.heads_per_kv = a.q_heads / a.kv_heads;
-  p.rows_kv = a.rows * p.heads_per_kv;
-  // scale 0 weighs every token alike: Q counts as zero
-  p.q_sign = a.scale > 0.f ? 1 : (a.scale < 0.f ? -1 : 0);
-  p.scale_log2 = p.q_sign == 0 ? 1.f : fabsf(a.scale) * 1.4426950408889634f;
-  p.vector_out = ((uintptr_t)a.out & 15) == 0 && a.o_bs % 8 == 0 && a.o_hs % 8 == 0 && a.o_ts % 8 == 0;
-  const bool slab = (1 << a.log2_group) == 16 * a.head_dim;
-  const int64_t need = chunk_tiles_bytes(a);
-  cudaError_t err;
-  if (need > 0) {
-    if (workspace_bytes < need) return AKV_ERR_INVALID;
-    ChunkSpace w;
-    space_layout(a, space_tiles(a), (uint8_t *)workspace, &w);
-    if (a.head_dim == 64) err = slab ? launch_tiles<64, true>(p, w) : launch_tiles<64, false>(p, w);
-    else err = slab ? launch_tiles<128, true>(p, w) : launch_tiles<128, false>(p, w);
-  } else {
-    if (a.head_dim == 64) err = slab ? launch_pages<64, true, 1>(p) : launch_pages<64, false, 1>(p);
-    else err = slab ? launch_pages<128, true, 1>(p) : launch_pages<128, false, 1>(p);
+int chunk_tiles_launch(const ChunkArgs &all, void *workspace, int64_t workspace_bytes) {
+  const int sms = device_sms();
+  if (sms <= 0) return AKV_ERR_CUDA;
+  if (workspace_bytes < chunk_tiles_bytes(all)) return AKV_ERR_INVALID;
+  const int step = slice_batch(all, sms);
+  for (int first = 0; first < all.batch; first += step) {
+    const ChunkArgs a = slice_of(all, first, std::min(step, all.batch - first));
+    ChunkParams p = {};
+    p.a = a;
+    p.heads_per_kv = a.q_heads / a.kv_heads;
+    p.rows_kv = a.rows * p.heads_per_kv;
+    p.fd_hpk = fast_div((uint32_t)p.heads_per_kv);
+    p.ctas = sms;
+    // scale 0 weighs every token alike: Q counts as zero
+    p.q_sign = a.scale > 0.f ? 1 : (a.scale < 0.f ? -1 : 0);
+    p.scale_log2 = p.q_sign == 0 ? 1.f : fabsf(a.scale) * 1.4426950408889634f;
+    p.vector_out = ((uintptr_t)a.out & 15) == 0 && a.o_bs % 8 == 0 && a.o_hs % 8 == 0 && a.o_ts % 8 == 0;
+    chunk_layout(a, sms, (uint8_t *)workspace, &p);
+    const bool slab = (1 << a.log2_group) == 16 * a.head_dim;
+    const cudaError_t err =
+        a.head_dim == 64 ? (slab ? launch_tiles<64, true>(p) : launch_tiles<64, false>(p))
+                         : (slab ? launch_tiles<128, true>(p) : launch_tiles<128, false>(p));
+    if (err != cudaSuccess) return AKV_ERR_CUDA;
   }
-  return err == cudaSuccess ? AKV_OK : AKV_ERR_CUDA;
+  return AKV_OK;
 }
 
 }  // namespace akv

@@ -127,26 +127,6 @@ __device__ __forceinline__ uint4 record_load8(int mode, const uint8_t *payload, 
 // within 2^-15 of a tie (about 1 chunk in 70 on random data) is redone with the
 // correctly rounded division.  No clamp is needed on the fast path: |y| <=
 // qmax + 0.07 rounds into [-qmax, qmax].
-__device__ __forceinline__ uint64_t f2_pack(float lo, float hi) {
-  return (uint64_t)__float_as_uint(lo) | ((uint64_t)__float_as_uint(hi) << 32);
-}
-__device__ __forceinline__ float f2_lo(uint64_t v) { return __uint_as_float((uint32_t)v); }
-__device__ __forceinline__ float f2_hi(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
-__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ uint64_t f2_sub(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 constexpr float kRoundMagic = 12582912.0f;  // 1.5 * 2^23
 constexpr float kTieGuard = 0.49996948242f;  // 0.5 - 2^-15
 

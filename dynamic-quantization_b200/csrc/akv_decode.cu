@@ -87,24 +87,6 @@ constexpr int64_t kHeaderBytes = 256;
 // Workspace: the header, then the partial states (kPartialsF holds their
 // offset in 4-byte words).
 
-// Division by a per-launch constant d for dividends 0 <= n < 2^31:
-// q = (umulhi(n, mul) + n) >> shift with shift = ceil(log2 d) and
-// mul = floor(2^32 (2^shift - d) / d) + 1 (Granlund and Montgomery, "Division
-// by invariant integers using multiplication", 1994).  Three instructions in
-// place of a runtime integer division.
-struct FastDiv {
-  uint32_t mul, shift;
-};
-__device__ __forceinline__ int fdiv(int n, FastDiv f) {
-  return (int)((__umulhi((uint32_t)n, f.mul) + (uint32_t)n) >> f.shift);
-}
-static FastDiv fast_div(uint32_t d) {  // d >= 1
-  uint32_t shift = 0;
-  while ((1ull << shift) < d) ++shift;
-  const uint64_t mul = ((1ull << 32) * ((1ull << shift) - d)) / d + 1;
-  return FastDiv{(uint32_t)mul, shift};
-}
-
 struct DecodeParams {
   const uint8_t *arena;
   int64_t arena_bytes;
@@ -1712,9 +1694,6 @@ static int visible_columns(int max_blocks, int rows, int heads_per_kv, int windo
   return *lead + (int)std::min<int64_t>(max_blocks - *lead, near);
 }
 
-// Whether a chunk of `rows_kv` rows per KV head runs on the tcgen05 tiles.
-static bool use_tiles(int64_t rows_kv) { return rows_kv > 8; }
-
 struct ChunkPlan {
   int rows_total;  // rows of all KV heads of a sequence
   int columns;     // page columns an item may see
@@ -1739,6 +1718,15 @@ static int chunk_plan(int batch, int rows, int q_heads, int kv_heads, int head_d
   r.sinks = sinks;
   return AKV_OK;
 }
+// Whether a chunk runs on tcgen05 tiles (akv_chunk.cu) or on the stream-K decode.
+// The decode dequantises every page once per 8 rows of its KV head; the tiles
+// unpack it once and then share it among 256 rows, but need four launches.  Measured
+// on a B200 with P pages x KV heads and g groups of 8 rows: the decode 15 us +
+// 0.85 ns P g, the tiles 45 us + (2.2 + 0.06 g) ns P.
+static bool use_tiles(const ChunkPlan &c, int batch, int kv_heads) {
+  const int64_t pages = (int64_t)batch * kv_heads * c.columns, groups = (c.rows_total / kv_heads + 7) / 8;
+  return pages * (groups - 4) > 40000;
+}
 }  // namespace akv
 
 extern "C" int64_t akv_chunk_workspace_bytes(int32_t batch, int32_t rows, int32_t q_heads, int32_t kv_heads,
@@ -1747,11 +1735,11 @@ extern "C" int64_t akv_chunk_workspace_bytes(int32_t batch, int32_t rows, int32_
   ChunkPlan c;
   Plan pl;
   if (chunk_plan(batch, rows, q_heads, kv_heads, head_dim, max_blocks, window, sinks, &c) != AKV_OK) return -1;
-  if (use_tiles(rows * c.rows.heads_per_kv)) {
+  if (use_tiles(c, batch, kv_heads)) {
     ChunkArgs a = {};
     a.columns = max_blocks, a.batch = batch, a.rows = rows, a.q_heads = q_heads, a.kv_heads = kv_heads;
     a.head_dim = head_dim, a.window = c.rows.window, a.lead = c.rows.lead;
-    return std::max(kHeaderBytes, chunk_tiles_bytes(a));
+    return chunk_tiles_bytes(a);
   }
   if (make_plan(batch, c.rows_total, kv_heads, head_dim, c.columns, splits, &pl) != AKV_OK) return -1;
   return pl.smax > kMaxSegments ? -1 : pl.bytes;
@@ -1768,15 +1756,15 @@ extern "C" int akv_chunk_attention(const void *arena, int64_t arena_bytes, const
   if (!out || q_token_stride % 8 || (!tokens && uniform_tokens < 0)) return AKV_ERR_INVALID;
   ChunkPlan c;
   if (int st = chunk_plan(batch, rows, q_heads, kv_heads, head_dim, max_blocks, window, sinks, &c)) return st;
+  if (group != 32 && group != 64 && group != 128 && group != 16 * head_dim) return AKV_ERR_UNSUPPORTED;
   c.rows.tokens = tokens;
   c.rows.uniform_tokens = std::min(uniform_tokens, kMaxTokens);
   c.rows.q_ts = q_token_stride;
   cudaStream_t s = (cudaStream_t)stream;
-  if (use_tiles(rows * c.rows.heads_per_kv)) {
+  if (use_tiles(c, batch, kv_heads)) {
     if (!arena || !table || !query || !workspace || ((uintptr_t)workspace & 15) || table_stride < max_blocks || arena_bytes < 0 || !isfinite(scale)) return AKV_ERR_INVALID;
     if (((uintptr_t)arena & 15) || ((uintptr_t)query & 15) || q_batch_stride % 8 || q_head_stride % 8) return AKV_ERR_INVALID;
     const int lg = ilog2_exact(group);
-    if (lg < 0 || (group != 32 && group != 64 && group != 128 && group != 16 * head_dim)) return AKV_ERR_UNSUPPORTED;
     ChunkArgs a = {};
     a.arena = (const uint8_t *)arena, a.arena_bytes = arena_bytes, a.table = table, a.table_stride = table_stride;
     a.seq_blocks = seq_blocks, a.columns = max_blocks, a.tokens = tokens, a.uniform_tokens = c.rows.uniform_tokens;

@@ -70,8 +70,8 @@ def test_window_decode_against_the_definition(cuda, case):
     scale = dim ** -0.5
     out = akv.packed_attention(q.to(cuda), store, scale, window=window, sinks=sinks)
     assert out.shape == q.shape and out.dtype == torch.float16
-    assert_rows_close(out, *attention_rows_f64(q, k, v, held, lengths, scale, window, sinks))
     assert akv.take_device_status(cuda) == 0
+    assert_rows_close(out, *attention_rows_f64(q, k, v, held, lengths, scale, window, sinks))
 
 
 CHUNKS = [
@@ -87,6 +87,13 @@ CHUNKS = [
     (128, 16, 1, 64, "page", [520], 71, 1, 0),
     (128, 4, 4, 2048, "tensor", [900, 60], 200, 5000, 7),
     (128, 72, 8, 2048, "tensor", [150, 33], 19, 40, 16),
+    # enough rows and pages for the tcgen05 tiles
+    (128, 8, 1, 2048, "tensor", [2500], 300, None, 0),
+    (128, 12, 4, 64, "page", [1700, 30, 900], 190, None, 0),
+    (64, 24, 8, 64, "page", [1200, 700], 150, 333, 37),
+    (64, 16, 4, 1024, "tensor", [1030, 2, 129, 1500], 257, 16, 1),
+    (128, 8, 8, 32, "page", [600, 590], 600, 200, 0),
+    (64, 6, 2, 128, "tensor", [4100], 700, 3000, 130),
 ]
 
 
@@ -99,5 +106,5 @@ def test_chunks_against_the_definition(cuda, case):
     scale = dim ** -0.5
     out = akv.chunk_attention(q.to(cuda), store, scale, window=window, sinks=sinks)
     assert out.shape == q.shape and out.dtype == torch.float16
-    assert_rows_close(out, *attention_rows_f64(q, k, v, held, lengths, scale, window, sinks))
     assert akv.take_device_status(cuda) == 0
+    assert_rows_close(out, *attention_rows_f64(q, k, v, held, lengths, scale, window, sinks))
