@@ -132,9 +132,13 @@ def require_cuda(tensor, what: str = "tensor") -> None:
 
 
 def stream_of(device) -> int:
+    """The current stream's handle on ``device`` (no stream object is made: this is on every call's path)."""
     import torch
 
-    return torch.cuda.current_stream(device).cuda_stream
+    index = getattr(device, "index", device)
+    if not isinstance(index, int):  # "cuda", or a device without an index: the current one
+        return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 class _Same:
@@ -155,7 +159,7 @@ def on_device(device):
     import torch
 
     index = device.index
-    return _SAME if index is None or index == torch.cuda.current_device() else torch.cuda.device(index)
+    return _SAME if index is None or index == torch._C._cuda_getDevice() else torch.cuda.device(index)
 
 
 DEV_BITS = {DEV_BAD_DESCRIPTOR: "a page descriptor outside the arena or misaligned (page skipped)",

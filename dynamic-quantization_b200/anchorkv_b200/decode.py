@@ -65,7 +65,7 @@ def _workspace(device: torch.device, nbytes: int, stream: int | None = None) -> 
     per stream forever).  Dropping one is safe: it was allocated on its own
     stream and used only there, so the allocator reuses its memory in that
     stream's order."""
-    if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+    if device.type == "cuda" and torch._C._cuda_isCurrentStreamCapturing():
         # a captured call's workspace belongs to its graph: one kept here would be
         # shared by every graph captured on this stream
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
@@ -113,6 +113,12 @@ def query_head_to_kv_head(query_head: int, *, num_query_heads: int, num_kv_heads
     return query_head // (num_query_heads // num_kv_heads)
 
 
+def _check_layout(layer) -> None:
+    if layer.dim not in (64, 128) or layer.block != 16 or not group_ok(layer.dim, layer.group):
+        raise ValueError('supported geometry: block=16, group=32/64/128 or one scale per '
+                         'block and head, head dim=64/128')
+
+
 def _check_query(query, layer, splits, *, empty_ok: bool) -> int:
     """The argument checks of triton_decode.py:86-94, in its order and with its
     messages, for a page table of ``layer``; returns the batch.
@@ -128,9 +134,7 @@ def _check_query(query, layer, splits, *, empty_ok: bool) -> int:
     length = layer.max_blocks if batched else layer.length
     if query.dtype != torch.float16 or not query.is_cuda or (length == 0 and not empty_ok):
         raise ValueError('packed kernel requires a nonempty CUDA FP16 cache')
-    if layer.dim not in (64, 128) or layer.block != 16 or not group_ok(layer.dim, layer.group):
-        raise ValueError('supported geometry: block=16, group=32/64/128 or one scale per '
-                         'block and head, head dim=64/128')
+    _check_layout(layer)
     if query.shape[1] % layer.heads:
         raise ValueError('query heads must be divisible by KV heads')
     if splits < 0:
@@ -190,9 +194,9 @@ def _check_window(window, sinks) -> None:
         raise ValueError("sinks must be non-negative and come with a window")
 
 
-def _layer_tokens(layer, batch, device):
-    """(int32 tensor or None, uniform count) of the tokens each sequence holds."""
-    tokens = layer.tokens if isinstance(layer, PagedBatch) else layer.length
+def _layer_tokens(layer, batched, batch, device):
+    """(device address or None, uniform count) of the tokens each sequence holds."""
+    tokens = layer.tokens if batched else layer.length
     if tokens is None:
         raise ValueError("the page table has no token counts (PagedBatch.over(pool, table, tokens=...)), so its "
                          "columns have no positions")
@@ -200,42 +204,46 @@ def _layer_tokens(layer, batch, device):
         if not 0 <= tokens < 1 << 31:
             raise ValueError("token counts must be non-negative 32-bit integers")
         return None, tokens
-    if tokens.dtype != torch.int32 or tuple(tokens.shape) != (batch,) or tokens.device != device \
-            or not tokens.is_contiguous():
+    if tokens.dtype != torch.int32 or tokens.shape != (batch,) or tokens.device != device or not tokens.is_contiguous():
         raise ValueError("tokens must be a contiguous int32 tensor [batch] on the query's device")
-    return tokens, 0
+    return tokens.data_ptr(), 0
 
 
 def _by_position(query, layer, scale, splits, window, sinks, out):
     """Attention of query rows that stand at the sequences' last positions."""
-    if out is not None and (out.dtype != torch.float16 or tuple(out.shape) != tuple(query.shape)
-                            or out.device != query.device or out.stride(-1) != 1):
-        raise ValueError("out must be an FP16 tensor of the query's shape on its device, unit stride in head_dim")
-    batch, heads, rows, dim = query.shape
-    dev = query.device
-    arena, arena_bytes, table, seq_blocks, max_blocks = _store_geometry(layer)
-    if arena.device != dev or table.device != dev:
-        raise ValueError("the query and the pages must be on one device")
-    tokens, uniform = _layer_tokens(layer, batch, dev)
+    shape, dev = query.shape, query.device
+    batch, heads, rows, dim = shape
     if out is None:
-        out = torch.empty(query.shape, dtype=query.dtype, device=dev)
-    if out.numel() == 0:
+        out = torch.empty(shape, dtype=torch.float16, device=dev)
+    elif out.dtype != torch.float16 or out.shape != shape or out.device != dev or out.stride(-1) != 1:
+        raise ValueError("out must be an FP16 tensor of the query's shape on its device, unit stride in head_dim")
+    batched = isinstance(layer, PagedBatch)
+    pool = layer.pool
+    table = layer.table if batched else layer.table.view(1, -1)
+    if pool.arena.device != dev or table.device != dev:
+        raise ValueError("the query and the pages must be on one device")
+    seq_blocks = layer.seq_blocks if batched else None
+    max_blocks = layer.max_blocks if batched else len(layer.pages)
+    tokens, uniform = _layer_tokens(layer, batched, batch, dev)
+    if rows == 0 or heads == 0 or batch == 0:
         return out
-    if query.stride(-1) != 1 or any(s % 8 for s in query.stride()[:-1]) or query.data_ptr() % 16:
+    qb, qh, qt, qd = query.stride()
+    if qd != 1 or (qb | qh | qt) & 7 or query.data_ptr() & 15:
         query = query.contiguous()
-    width = min(window, 1 << 30) if window is not None else 0
+        qb, qh, qt, _ = query.stride()
+    width = 0 if window is None else min(window, 1 << 30)
     sinks = min(sinks, 1 << 30)
+    ob, oh, ot, _ = out.stride()
     with _lib.on_device(dev):
-        nbytes = _chunk_bytes(dev, batch, rows, heads, layer.heads, dim, max_blocks, width, sinks, splits)
+        nbytes = _chunk_bytes(dev, batch, rows, heads, pool.heads, dim, max_blocks, width, sinks, splits)
         if nbytes < 0:
             raise ValueError('unsupported decode geometry')
         stream = _lib.stream_of(dev)
         ws = _workspace(dev, nbytes, stream)
-        _lib.call("akv_chunk_attention", arena.data_ptr(), arena_bytes, table.data_ptr(), table.stride(0),
-                  None if seq_blocks is None else seq_blocks.data_ptr(), max_blocks,
-                  None if tokens is None else tokens.data_ptr(), uniform, query.data_ptr(), *query.stride()[:3],
-                  batch, rows, heads, layer.heads, dim, layer.group, float(scale), width, sinks, splits,
-                  out.data_ptr(), *out.stride()[:3], ws.data_ptr(), ws.numel(), _lib.status_ptr(dev), stream)
+        _lib.call("akv_chunk_attention", pool.arena.data_ptr(), pool.nbytes, table.data_ptr(), table.stride(0),
+                  None if seq_blocks is None else seq_blocks.data_ptr(), max_blocks, tokens, uniform,
+                  query.data_ptr(), qb, qh, qt, batch, rows, heads, pool.heads, dim, pool.group, scale, width, sinks,
+                  splits, out.data_ptr(), ob, oh, ot, ws.data_ptr(), ws.numel(), _lib.status_ptr(dev), stream)
     return out
 
 
@@ -258,10 +266,16 @@ def chunk_attention(query, layer, scale, *, window=None, sinks=0, out=None):
     other rows of the call."""
     layer = _as_table(layer)
     batched = isinstance(layer, PagedBatch)
-    if query.dim() != 4 or query.shape[0] != (layer.batch if batched else 1) or query.shape[-1] != layer.dim:
+    shape = query.shape
+    if len(shape) != 4 or shape[0] != (layer.batch if batched else 1) or shape[3] != layer.dim:
         raise ValueError('query must be [batch, heads, rows, head_dim] for the page table')
-    _check_query(query[:, :, :1], layer, 0, empty_ok=False)
-    _check_window(window, sinks)
+    if query.dtype != torch.float16 or not query.is_cuda or (layer.max_blocks if batched else layer.length) == 0:
+        raise ValueError('packed kernel requires a nonempty CUDA FP16 cache')
+    _check_layout(layer)
+    if shape[1] % layer.heads:
+        raise ValueError('query heads must be divisible by KV heads')
+    if window is not None or sinks:
+        _check_window(window, sinks)
     return _by_position(query, layer, scale, _CHUNK_SPLITS, window, sinks, out)
 
 

@@ -124,9 +124,10 @@ class _FreeSlots:
     then the runs in ascending order."""
 
     __slots__ = ("_stack", "_top", "_runs", "_in_runs")
+    _NONE = np.zeros(0, np.int64)
 
     def __init__(self):
-        self._stack, self._top = np.zeros(0, np.int64), 0
+        self._stack, self._top = self._NONE, 0
         self._runs, self._in_runs = [], 0
 
     def __len__(self) -> int:
@@ -179,6 +180,17 @@ class _FreeSlots:
         self._top = need
 
 
+_PAGE_BYTES: dict = {}
+
+
+def _page_bytes(heads: int, dim: int, group: int) -> dict:
+    """Bytes of a page by precision, one dict per geometry."""
+    key = (heads, dim, group)
+    if key not in _PAGE_BYTES:
+        _PAGE_BYTES[key] = {b: heads * record_bytes(dim, group, b) for b in (4, 8, 16)}
+    return _PAGE_BYTES[key]
+
+
 class PagePool:
     """An arena of page slots in three size classes (FP16 / INT8 / INT4).
 
@@ -210,8 +222,8 @@ class PagePool:
 
     def _lay_out(self, heads: int, dim: int, group: int, pages: dict | None) -> None:
         self.heads, self.dim, self.group = heads, dim, group
-        pages = dict(pages or {})
-        self.page_bytes = {b: heads * record_bytes(dim, group, b) for b in (4, 8, 16)}
+        pages = pages or {}
+        self.page_bytes = _page_bytes(heads, dim, group)
         self.base, self.capacity, self._free = {}, {}, {}
         cursor = 0
         for bits in (16, 8, 4):

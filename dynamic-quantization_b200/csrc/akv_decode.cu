@@ -312,10 +312,10 @@ struct SoftmaxState {
   float m0, m1, l0, l1;  // heads 2t4, 2t4+1: running max (base 2) and this lane's sum
 };
 
-// What the rows of one item of a multi-row decode see: row n (lane rows 2t4,
-// 2t4+1 here) stands at token position at0 / at1 and sees positions up to its
-// own that lie less than `window` tokens back or below `sinks`; at_lo and at_hi
-// are the item's lowest and highest row positions.
+// What the rows of one item of a multi-row decode see: row n (lane rows 2t4, 2t4+1
+// here) stands at token position at0 / at1 and sees positions up to its own that lie
+// less than `window` tokens back or below `sinks`; at_lo and at_hi are the item's
+// lowest and highest row positions.  Only pages at the borders of what they see ask.
 struct RowView {
   int at0, at1, at_lo, at_hi, window, sinks;
   __device__ __forceinline__ bool sees(int at, int pos) const {
@@ -326,10 +326,12 @@ struct RowView {
   __device__ __forceinline__ bool any(int pos) const {
     return pos <= at_hi && (pos > at_lo - window || pos < sinks);
   }
-  // Whether every row of the item sees all 16 tokens of page column `col`.
-  __device__ __forceinline__ bool whole_page(int col) const {
-    const int p0 = kBlock * col, p1 = p0 + kBlock - 1;
-    return p1 <= at_lo && (p0 > at_hi - window || p1 < sinks);
+  // pages_softmax's bits for the lane's scores of a page.
+  __device__ __forceinline__ uint32_t hidden(int col, int ntok, int gid) const {
+    const int pos = kBlock * col + gid;
+    const bool low = gid < ntok, high = gid + 8 < ntok;
+    return (low && sees(at0, pos) ? 0u : 1u) | (low && sees(at1, pos) ? 0u : 2u) |
+           (high && sees(at0, pos + 8) ? 0u : 4u) | (high && sees(at1, pos + 8) ? 0u : 8u);
   }
 };
 
@@ -339,12 +341,12 @@ struct RowView {
 // exceeds it by more than 2^8 (P <= 2^8 stays exact enough in fp16 and most
 // pages need no reduction).  With NP = 2 the second page is skipped when `two`
 // is false.
-// ROWS: `part[r]` says that some row does not see all of page r (column col[r]).
+// ROWS: bit 4 r + i of `hide` hides score i of page r from its row; `ntok` is not looked at.
 template <int D, int NP, bool ROWS>
 __device__ __forceinline__ void pages_softmax(float (&s)[NP][4], const int (&ntok)[NP], bool two,
                                               int gid, float scale_log2, SoftmaxState &st,
                                               float (&o)[D / 16][4], uint32_t (&b)[NP][2],
-                                              const bool (&part)[NP], const int (&col)[NP], const RowView &view) {
+                                              bool partial, uint32_t hide) {
   constexpr float slack = 8.f;
   constexpr float kNegInf = -INFINITY;
   float x[NP][4];
@@ -353,18 +355,15 @@ __device__ __forceinline__ void pages_softmax(float (&s)[NP][4], const int (&nto
   for (int r = 0; r < NP; ++r) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[r][i] = s[r][i] * scale_log2;
-    if (ntok[r] < kBlock) {  // tokens past the page's valid count do not exist
+    if constexpr (ROWS) {
+      if (partial) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if ((hide >> (4 * r + i)) & 1u) x[r][i] = kNegInf;
+      }
+    } else if (ntok[r] < kBlock) {  // tokens past the page's valid count do not exist
       if (gid >= ntok[r]) x[r][0] = x[r][1] = kNegInf;
       if (gid + 8 >= ntok[r]) x[r][2] = x[r][3] = kNegInf;
-    }
-    if constexpr (ROWS) {
-      if (part[r]) {
-        const int pos = kBlock * col[r] + gid;
-        if (!view.sees(view.at0, pos)) x[r][0] = kNegInf;
-        if (!view.sees(view.at1, pos)) x[r][1] = kNegInf;
-        if (!view.sees(view.at0, pos + 8)) x[r][2] = kNegInf;
-        if (!view.sees(view.at1, pos + 8)) x[r][3] = kNegInf;
-      }
     }
     mx0 = fmaxf(mx0, fmaxf(x[r][0], x[r][2]));
     mx1 = fmaxf(mx1, fmaxf(x[r][1], x[r][3]));
@@ -400,6 +399,32 @@ __device__ __forceinline__ void pages_softmax(float (&s)[NP][4], const int (&nto
   }
 }
 
+// The row positions of an item of a multi-row decode, and its query-head group.
+struct ItemRows {
+  int held, at_first, row0, n, at_lo, at_hi;  // pages; position of query token 0; first row of the group, its rows
+};
+__device__ __forceinline__ ItemRows item_rows(const DecodeParams &p, int item) {
+  ItemRows v;
+  const int b = fdiv(item, p.fd_ipb);
+  v.held = p.seq_blocks ? max(0, min(__ldg(p.seq_blocks + b), p.columns)) : p.columns;
+  const int tokens = min(p.tokens ? __ldg(p.tokens + b) : p.uniform_tokens, kBlock * v.held);
+  v.at_first = tokens - p.rows;
+  v.row0 = 8 * (item - fdiv(item, p.fd_qgroups) * p.qgroups);  // items are kv_heads * qgroups per sequence
+  v.n = min(8, p.gqa - v.row0);
+  v.at_lo = v.at_first + fdiv(v.row0, p.fd_hpk);
+  v.at_hi = v.at_first + fdiv(v.row0 + v.n - 1, p.fd_hpk);
+  return v;
+}
+__device__ __forceinline__ RowView row_view(const DecodeParams &p, int item, int t4) {
+  const ItemRows v = item_rows(p, item);
+  RowView r;
+  // Rows past the group's count repeat its last row: they only waste a lane.
+  r.at0 = v.at_first + fdiv(v.row0 + min(2 * t4, v.n - 1), p.fd_hpk);
+  r.at1 = v.at_first + fdiv(v.row0 + min(2 * t4 + 1, v.n - 1), p.fd_hpk);
+  r.at_lo = v.at_lo, r.at_hi = v.at_hi, r.window = p.window, r.sinks = p.sinks;
+  return r;
+}
+
 // Zero the V rows past a partial page's valid count, so that P = 0 never meets
 // a non-finite value.  The V payload is swizzled inside 128-byte lines, which
 // may hold several rows: every word from the line of row `ntok` on is zeroed
@@ -431,14 +456,16 @@ __device__ __forceinline__ void zero_unseen(uint8_t *rec, int ntok, int col, con
 template <int D, bool SLAB, bool ROWS>
 __device__ __forceinline__ void fp16_attend(uint8_t *rec, int ntok, int lane, const ScaleIdx &si,
                                             const uint32_t (&qf)[D / 16][2], float scale_log2,
-                                            SoftmaxState &st, float (&o)[D / 16][4], int col0, const RowView &view) {
+                                            SoftmaxState &st, float (&o)[D / 16][4], const DecodeParams &p, int item,
+                                            bool partial, int2 cols) {
   constexpr int PB = kBlock * D * 2;
   const int gid = lane >> 2, t4 = lane & 3;
-  const int col[1] = {col0};
-  const bool part[1] = {ROWS && !view.whole_page(col0)};
+  uint32_t hide = 0;
   if constexpr (ROWS) {
-    if (ntok < kBlock || part[0]) {
-      zero_unseen<D, AKV_MODE_FP16>(rec, ntok, col0, view, lane);
+    if (partial) {
+      const RowView view = row_view(p, item, t4);
+      hide = view.hidden(cols.x, ntok, gid);
+      zero_unseen<D, AKV_MODE_FP16>(rec, ntok, cols.x, view, lane);
       __syncwarp();
     }
   } else if (ntok < kBlock) {
@@ -450,7 +477,7 @@ __device__ __forceinline__ void fp16_attend(uint8_t *rec, int ntok, int lane, co
   uint32_t b[1][2];
   const int nt[1] = {ntok};
   page_qk<D, AKV_MODE_FP16, SLAB>(rec, nullptr, none, gid, t4, qf, s[0]);
-  pages_softmax<D, 1, ROWS>(s, nt, false, gid, scale_log2, st, o, b, part, col, view);
+  pages_softmax<D, 1, ROWS>(s, nt, false, gid, scale_log2, st, o, b, partial, hide);
   page_pv<D, AKV_MODE_FP16, SLAB>(rec + PB, nullptr, si, gid, t4, b[0][0], b[0][1], o);
 }
 
@@ -469,17 +496,21 @@ template <int D, int MODE, bool SLAB, bool ROWS>
 __device__ __forceinline__ void slot_attend(uint8_t *rec, uint32_t rb, bool has2, int ntok0,
                                             int ntok1, int lane, int log2_group, const ScaleIdx &si,
                                             const uint32_t (&qf)[D / 16][2], float scale_log2,
-                                            SoftmaxState &st, float (&o)[D / 16][4], int col0, int col1,
-                                            const RowView &view) {
+                                            SoftmaxState &st, float (&o)[D / 16][4], const DecodeParams &p, int item,
+                                            bool partial, int2 cols) {
   constexpr int PB = kBlock * D * mode_bits(MODE) / 8;
   const int gid = lane >> 2, t4 = lane & 3;
   const int npages = has2 ? 2 : 1;
-  const int col[2] = {col0, col1};
-  const bool part[2] = {ROWS && !view.whole_page(col0), ROWS && has2 && !view.whole_page(col1)};
+  uint32_t hide = 0;
   if constexpr (ROWS) {
-    if (ntok0 < kBlock || part[0] || (has2 && (ntok1 < kBlock || part[1]))) {
-      zero_unseen<D, MODE>(rec, ntok0, col0, view, lane);
-      if (has2) zero_unseen<D, MODE>(rec + rb, ntok1, col1, view, lane);
+    if (partial) {
+      const RowView view = row_view(p, item, t4);
+      hide = view.hidden(cols.x, ntok0, gid);
+      zero_unseen<D, MODE>(rec, ntok0, cols.x, view, lane);
+      if (has2) {
+        hide |= view.hidden(cols.y, ntok1, gid) << 4;
+        zero_unseen<D, MODE>(rec + rb, ntok1, cols.y, view, lane);
+      }
       __syncwarp();
     }
   } else if (ntok0 < kBlock || (has2 && ntok1 < kBlock)) {
@@ -507,7 +538,7 @@ __device__ __forceinline__ void slot_attend(uint8_t *rec, uint32_t rb, bool has2
   }
   const int nt[2] = {ntok0, has2 ? ntok1 : 0};
   uint32_t b[2][2];
-  pages_softmax<D, 2, ROWS>(s, nt, has2, gid, scale_log2, st, o, b, part, col, view);
+  pages_softmax<D, 2, ROWS>(s, nt, has2, gid, scale_log2, st, o, b, partial, hide);
   if constexpr (MODE == AKV_MODE_INT4) {
     page_pv<D, MODE, SLAB>(rec + PB, reinterpret_cast<const __half *>(rec + 2 * PB) + vgap, si, gid, t4,
                                  b[0][0], b[0][1], o);
@@ -562,32 +593,6 @@ __device__ __forceinline__ void query_fragments(const uint32_t (&qw)[D / 8], uin
     qf[c][0] = prmt(qw[4 * j + hb], qw[4 * j + 2 + hb], 0x5410);
     qf[c][1] = prmt(qw[4 * j + hb], qw[4 * j + 2 + hb], 0x7632);
   }
-}
-
-// The row positions of an item of a multi-row decode, and its query-head group.
-struct ItemRows {
-  int at_first, row0, n, at_lo, at_hi;  // position of query token 0; first row of the group, its rows
-};
-__device__ __forceinline__ ItemRows item_rows(const DecodeParams &p, int item) {
-  ItemRows v;
-  const int b = fdiv(item, p.fd_ipb);
-  const int held = kBlock * (p.seq_blocks ? max(0, min(__ldg(p.seq_blocks + b), p.columns)) : p.columns);
-  const int tokens = min(p.tokens ? __ldg(p.tokens + b) : p.uniform_tokens, held);
-  v.at_first = tokens - p.rows;
-  v.row0 = 8 * (item - fdiv(item, p.fd_qgroups) * p.qgroups);  // items are kv_heads * qgroups per sequence
-  v.n = min(8, p.gqa - v.row0);
-  v.at_lo = v.at_first + fdiv(v.row0, p.fd_hpk);
-  v.at_hi = v.at_first + fdiv(v.row0 + v.n - 1, p.fd_hpk);
-  return v;
-}
-__device__ __forceinline__ RowView row_view(const DecodeParams &p, int item, int t4) {
-  const ItemRows v = item_rows(p, item);
-  RowView r;
-  // Rows past the group's count repeat its last row: they only waste a lane.
-  r.at0 = v.at_first + fdiv(v.row0 + min(2 * t4, v.n - 1), p.fd_hpk);
-  r.at1 = v.at_first + fdiv(v.row0 + min(2 * t4 + 1, v.n - 1), p.fd_hpk);
-  r.at_lo = v.at_lo, r.at_hi = v.at_hi, r.window = p.window, r.sinks = p.sinks;
-  return r;
 }
 
 // SLAB: one scale per 16-token slab (group = 16 * head_dim), the
@@ -668,13 +673,14 @@ __global__ void __launch_bounds__(DecodeTraits<D>::kMaxThreads, 1)
     nb = 0;
     if (e < e_end) {
       const int it = fdiv(e, p.fd_mb), bb = fdiv(it, p.fd_ipb);
-      if constexpr (ROWS) {  // nb: the entry's column, raw a skip entry where the item sees nothing of it
+      if constexpr (ROWS) {  // nb: the entry's column, negative where some row does not see the whole page;
+                             // raw: a skip entry where the item sees nothing of it
         const ItemRows v = item_rows(p, it);
         const int first = max(p.lead, max(v.at_lo - p.window + 1, 0) / kBlock);
-        const int j = e - it * mb;
-        nb = j < p.lead ? j : first + (j - p.lead);
-        const int held = p.seq_blocks ? min(__ldg(p.seq_blocks + bb), p.columns) : p.columns;
-        if (nb < held && kBlock * nb <= v.at_hi) raw = __ldg(p.table + (int64_t)bb * p.table_stride + nb);
+        const int j = e - it * mb, col = j < p.lead ? j : first + (j - p.lead), pos = kBlock * col;
+        if (col < v.held && pos <= v.at_hi) raw = __ldg(p.table + (int64_t)bb * p.table_stride + col);
+        const bool whole = pos + kBlock - 1 <= v.at_lo && (pos > v.at_hi - p.window || pos + kBlock - 1 < p.sinks);
+        nb = col | (whole ? 0 : (int)0x80000000);
       } else {
         nb = p.seq_blocks ? min(__ldg(p.seq_blocks + bb), mb) : mb;
         raw = __ldg(p.table + (int64_t)bb * p.table_stride + (e - it * mb));
@@ -697,7 +703,6 @@ __global__ void __launch_bounds__(DecodeTraits<D>::kMaxThreads, 1)
       const int it = fdiv(e, p.fd_mb), j = e - it * mb;
       first = j == 0;
       mode = ROWS || j < nb ? desc_mode(raw) : AKV_MODE_SKIP;
-      if constexpr (ROWS) w_col = nb;
       rb = mode == AKV_MODE_FP16 ? rb16 : (mode == AKV_MODE_INT8 ? rb8 : rb4);
       const int64_t poff = desc_offset(raw);
       ok = mode != AKV_MODE_SKIP;
@@ -707,6 +712,10 @@ __global__ void __launch_bounds__(DecodeTraits<D>::kMaxThreads, 1)
       }
       w_src = poff + (int64_t)fdiv(it - fdiv(it, p.fd_ipb) * ipb, p.fd_qgroups) * rb;
       w_meta = (uint32_t)mode | ((uint32_t)desc_ntok(raw) << 4) | ((uint32_t)(it - first_item) << 16);
+      if constexpr (ROWS) {  // bit 3: some row does not see all of the page
+        w_col = nb & 0x7fffffff;
+        w_meta |= nb < 0 || desc_ntok(raw) < kBlock ? 8u : 0u;
+      }
     }
     // An INT8 or INT4 page pairs with the next page of its item and mode in
     // the window: in each (item, mode) group of lanes the 1st and 2nd pages
@@ -728,7 +737,7 @@ __global__ void __launch_bounds__(DecodeTraits<D>::kMaxThreads, 1)
     if constexpr (ROWS) w_col2 = __shfl_sync(0xffffffffu, w_col, partner);
     const uint32_t pmeta = __shfl_sync(0xffffffffu, w_meta, partner);
     w_need = partner != lane ? 2u * rb : rb;
-    if (partner != lane) w_meta |= 4u | (((pmeta >> 4) & 31u) << 9);
+    if (partner != lane) w_meta |= 4u | (((pmeta >> 4) & 31u) << 9) | (ROWS ? pmeta & 8u : 0u);
     w_mask = __ballot_sync(0xffffffffu, ok && !follower);
   };
   int win0 = e_begin;
@@ -756,8 +765,6 @@ __global__ void __launch_bounds__(DecodeTraits<D>::kMaxThreads, 1)
 #pragma unroll
   for (int m = 0; m < T::kTiles; ++m) o[m][0] = o[m][1] = o[m][2] = o[m][3] = 0.f;
   SoftmaxState st{-INFINITY, -INFINITY, 0.f, 0.f};
-  RowView view{};
-  if constexpr (ROWS) view = row_view(p, first_item, t4);
   int cur_seg = 0;
 
   auto finalize = [&](int seg) {
@@ -797,7 +804,6 @@ __global__ void __launch_bounds__(DecodeTraits<D>::kMaxThreads, 1)
       uint32_t qw[D / 8];
       load_query<D, ROWS>(p, first_item + cur_seg, gid, t4, qw);
       query_fragments<D>(qw, qf);
-      if constexpr (ROWS) view = row_view(p, first_item + cur_seg, t4);
     }
   };
 
@@ -865,19 +871,21 @@ __global__ void __launch_bounds__(DecodeTraits<D>::kMaxThreads, 1)
     }
     const int ntok = (int)((meta >> 4) & 31), ntok1 = (int)((meta >> 9) & 31);
     const bool has2 = (meta & 4u) != 0;
+    const bool partial = ROWS && (meta & 8u);
     int2 cols = make_int2(0, 0);
-    if constexpr (ROWS) cols = slot_cols[slot];
+    if (partial) cols = slot_cols[slot];
+    const int item = first_item + cur_seg;
     switch (meta & 3u) {
       case AKV_MODE_INT4:
         slot_attend<D, AKV_MODE_INT4, SLAB, ROWS>(rec, rb4, has2, ntok, ntok1, lane, lg, si, qf, p.scale_log2, st, o,
-                                                  cols.x, cols.y, view);
+                                                  p, item, partial, cols);
         break;
       case AKV_MODE_INT8:
         slot_attend<D, AKV_MODE_INT8, SLAB, ROWS>(rec, rb8, has2, ntok, ntok1, lane, lg, si, qf, p.scale_log2, st, o,
-                                                  cols.x, cols.y, view);
+                                                  p, item, partial, cols);
         break;
       default:
-        fp16_attend<D, SLAB, ROWS>(rec, ntok, lane, si, qf, p.scale_log2, st, o, cols.x, view);
+        fp16_attend<D, SLAB, ROWS>(rec, ntok, lane, si, qf, p.scale_log2, st, o, p, item, partial, cols);
         break;
     }
     __syncwarp();
