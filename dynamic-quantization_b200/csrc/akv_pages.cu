@@ -26,13 +26,13 @@ static PageBytes page_bytes(int heads, int head_dim, int group) {
 
 constexpr int kCopyThreads = 256;
 
-// Copy 16-byte units [lo, hi) of a page by one CTA; four loads of a thread are in
-// flight before the first is stored.
-__device__ __forceinline__ void copy_units(const uint8_t *src, uint8_t *dst, int64_t lo, int64_t hi) {
+// Copy 16-byte units [lo, hi) of a page by one CTA, U loads of a thread in flight
+// before the first is stored.
+template <int U>
+__device__ __forceinline__ void copy_units(const uint8_t *src, uint8_t *dst, int lo, int hi) {
   const uint4 *s = reinterpret_cast<const uint4 *>(src);
   uint4 *d = reinterpret_cast<uint4 *>(dst);
-  constexpr int U = 4;
-  for (int64_t i = lo + threadIdx.x; i < hi; i += U * kCopyThreads) {
+  for (int i = lo + (int)threadIdx.x; i < hi; i += U * kCopyThreads) {
     uint4 v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -61,11 +61,14 @@ struct ForkParams {
 // and copies its share of the page that the child's next token goes to, when
 // that page is half filled and the child was given a fresh slot.
 __global__ void __launch_bounds__(kCopyThreads) fork_pages_kernel(const ForkParams p) {
+  grid_dependency_wait();
+  allow_dependents_launch();
   const int part = blockIdx.x % p.parts;
   const int64_t row = blockIdx.x / p.parts;  // layer * children + child
   const int child = (int)(row % p.children);
   const int64_t layer = row / p.children;
   int64_t *out = p.out + row * p.columns;
+  const int64_t fresh = p.fresh ? p.fresh[row] : 0;
   const int c0 = (int)((int64_t)p.columns * part / p.parts), c1 = (int)((int64_t)p.columns * (part + 1) / p.parts);
   const int64_t parent = p.parents[child];
   if (parent < 0 || parent >= p.batch) {  // no such sequence: an empty row
@@ -75,7 +78,6 @@ __global__ void __launch_bounds__(kCopyThreads) fork_pages_kernel(const ForkPara
   }
   const int64_t *src_row = p.table + layer * p.layer_stride + parent * p.seq_stride;
   const int tokens = p.tokens ? p.tokens[parent] : p.uniform_tokens;
-  const int64_t fresh = p.fresh ? p.fresh[row] : 0;
   int copied = -1;  // the column whose page is copied
   int64_t old = 0;
   if (fresh != 0 && tokens > 0 && tokens % kBlock != 0 && tokens / kBlock < p.columns) {
@@ -93,8 +95,8 @@ __global__ void __launch_bounds__(kCopyThreads) fork_pages_kernel(const ForkPara
     out[c] = c == copied ? (fresh & ~(int64_t)255) | (old & 255) : src_row[c];
   if (copied < 0) return;
   const int64_t units = p.bytes(desc_mode(old)) / 16;
-  copy_units(p.arena + desc_offset(old), p.arena + desc_offset(fresh), units * part / p.parts,
-             units * (part + 1) / p.parts);
+  copy_units<8>(p.arena + desc_offset(old), p.arena + desc_offset(fresh), (int)(units * part / p.parts),
+             (int)(units * (part + 1) / p.parts));
 }
 
 // ================================================================= compact
@@ -106,6 +108,8 @@ __global__ void __launch_bounds__(kCopyThreads) fork_pages_kernel(const ForkPara
 //   rank   an owner's rank is the owners before it; place[key] = its new offset;
 //   move   owners copy their page, every entry is rewritten through place[key].
 constexpr int kRankThreads = 1024;
+// Entries that one CTA plans: 8192 take it about 8 us, the four kernels' launches cost more.
+constexpr int kOnePlan = 8192;
 
 struct CompactParams {
   const int64_t *table;
@@ -130,6 +134,7 @@ __device__ __forceinline__ bool movable(const CompactParams &p, int64_t d) {
 }
 
 __global__ void __launch_bounds__(256) compact_mark_kernel(const CompactParams p) {
+  allow_dependents_launch();
   for (int64_t e = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; e < p.n; e += (int64_t)gridDim.x * blockDim.x) {
     const int64_t d = p.table[e];
     if (movable(p, d)) atomicMin(p.owner + desc_offset(d) / p.unit, (uint32_t)e);
@@ -137,13 +142,44 @@ __global__ void __launch_bounds__(256) compact_mark_kernel(const CompactParams p
   }
 }
 
+// The rank of this thread's entry among the owners of its precision within the CTA
+// (mode 0: none), and how many each precision has there.
+__device__ __forceinline__ int block_rank(int mode, int (&warps)[4][32], int (&all)[4]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int rank = 0;
+#pragma unroll
+  for (int m = 1; m < 4; ++m) {
+    const uint32_t mask = __ballot_sync(0xffffffffu, mode == m);
+    if (mode == m) rank = __popc(mask & ((1u << lane) - 1u));
+    if (lane == 0) warps[m][warp] = __popc(mask);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int m = 1; m < 4; ++m) {
+    const int n = warps[m][lane];
+    const int before = __reduce_add_sync(0xffffffffu, lane < warp ? n : 0);
+    all[m] = __reduce_add_sync(0xffffffffu, n);
+    if (mode == m) rank += before;
+  }
+  __syncthreads();
+  return rank;
+}
+__device__ __forceinline__ void set_place(const CompactParams &p, int64_t d, int rank) {
+  const int mode = desc_mode(d);
+  const bool fits = rank < p.capacity[mode];  // else: more pages than the target holds, skip entries
+  if (!fits) set_status(p.status, AKV_DEV_BAD_DESCRIPTOR);
+  p.place[desc_offset(d) / p.unit] = fits ? p.base[mode] + rank * p.bytes(mode) : -1;
+}
+
 // The mode of entry e when it is the first to name its page, else 0.
 __device__ __forceinline__ int owner_mode(const CompactParams &p, int64_t e, int64_t &d) {
   d = e < p.n ? p.table[e] : 0;
-  return movable(p, d) && p.owner[desc_offset(d) / p.unit] == (uint32_t)e ? desc_mode(d) : 0;
+  return movable(p, d) && __ldcg(p.owner + desc_offset(d) / p.unit) == (uint32_t)e ? desc_mode(d) : 0;
 }
 
 __global__ void __launch_bounds__(kRankThreads) compact_count_kernel(const CompactParams p) {
+  grid_dependency_wait();
+  allow_dependents_launch();
   int64_t d;
   const int mode = owner_mode(p, blockIdx.x * (int64_t)kRankThreads + threadIdx.x, d);
 #pragma unroll
@@ -155,52 +191,83 @@ __global__ void __launch_bounds__(kRankThreads) compact_count_kernel(const Compa
 
 __global__ void __launch_bounds__(kRankThreads) compact_rank_kernel(const CompactParams p) {
   __shared__ int before[4], warps[4][32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  grid_dependency_wait();
+  allow_dependents_launch();
   if (threadIdx.x < 4) before[threadIdx.x] = 0;
   __syncthreads();
   // owners of each precision in the blocks before this one
   int sum[4] = {0, 0, 0, 0};
   for (int b = threadIdx.x; b < (int)blockIdx.x; b += kRankThreads)
 #pragma unroll
-    for (int m = 1; m < 4; ++m) sum[m] += p.counts[4 * b + m];
+    for (int m = 1; m < 4; ++m) sum[m] += __ldcg(p.counts + 4 * b + m);
 #pragma unroll
   for (int m = 1; m < 4; ++m) {
     const int s = __reduce_add_sync(0xffffffffu, sum[m]);
-    if (lane == 0 && s) atomicAdd(&before[m], s);  // integers: any order gives the same sum
+    if ((threadIdx.x & 31) == 0 && s) atomicAdd(&before[m], s);  // integers: any order gives the same sum
   }
   int64_t d;
   const int mode = owner_mode(p, blockIdx.x * (int64_t)kRankThreads + threadIdx.x, d);
-  int rank = 0;
+  int all[4];
+  const int rank = block_rank(mode, warps, all);
+  if (mode != 0) set_place(p, d, before[mode] + rank);
+}
+
+// Small tables: all of the plan in one CTA, which saves three launches.
+__global__ void __launch_bounds__(kRankThreads) compact_plan_kernel(const CompactParams p, int keys) {
+  __shared__ int warps[4][32];
+  grid_dependency_wait();
+  allow_dependents_launch();
+  uint4 *owner = reinterpret_cast<uint4 *>(p.owner);
+  for (int k = threadIdx.x; k < (keys + 3) / 4; k += kRankThreads) owner[k] = make_uint4(~0u, ~0u, ~0u, ~0u);
+  __syncthreads();
+  constexpr int N = kOnePlan / kRankThreads;  // entries of a thread, their loads in flight together
+  int64_t d[N];
+  int64_t key[N];
 #pragma unroll
-  for (int m = 1; m < 4; ++m) {
-    const uint32_t mask = __ballot_sync(0xffffffffu, mode == m);
-    if (mode == m) rank = __popc(mask & ((1u << lane) - 1u));
-    if (lane == 0) warps[m][warp] = __popc(mask);
+  for (int i = 0; i < N; ++i) {
+    const int e = i * kRankThreads + threadIdx.x;
+    d[i] = e < (int)p.n ? p.table[e] : 0;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    key[i] = -1;
+    if (movable(p, d[i])) {
+      key[i] = desc_offset(d[i]) / p.unit;
+      atomicMin(p.owner + key[i], (uint32_t)(i * kRankThreads + threadIdx.x));
+    } else if (desc_mode(d[i]) != AKV_MODE_SKIP) {
+      set_status(p.status, AKV_DEV_BAD_DESCRIPTOR);
+    }
   }
   __syncthreads();
-  if (mode == 0) return;
-  for (int w = 0; w < warp; ++w) rank += warps[mode][w];
-  rank += before[mode];
-  const int64_t key = desc_offset(d) / p.unit;
-  if (rank >= p.capacity[mode]) {  // more pages than the target holds: the entries become skip entries
-    set_status(p.status, AKV_DEV_BAD_DESCRIPTOR);
-    p.place[key] = -1;
-  } else {
-    p.place[key] = p.base[mode] + rank * p.bytes(mode);
+  uint32_t first[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) first[i] = key[i] >= 0 ? __ldcg(p.owner + key[i]) : ~0u;
+  int before[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (i * kRankThreads >= (int)p.n) break;
+    const int mode = first[i] == (uint32_t)(i * kRankThreads + threadIdx.x) ? desc_mode(d[i]) : 0;
+    int all[4];
+    const int rank = block_rank(mode, warps, all);
+    if (mode != 0) set_place(p, d[i], before[mode] + rank);
+#pragma unroll
+    for (int m = 1; m < 4; ++m) before[m] += all[m];
   }
 }
 
 // One CTA per table entry.
 __global__ void __launch_bounds__(kCopyThreads) compact_move_kernel(const CompactParams p) {
   const int64_t e = blockIdx.x;
+  grid_dependency_wait();
+  allow_dependents_launch();
   const int64_t d = p.table[e];
   if (!movable(p, d)) {
     if (threadIdx.x == 0) p.out[e] = 0;
     return;
   }
   const int64_t key = desc_offset(d) / p.unit;
-  const uint32_t owner = p.owner[key];
-  const int64_t place = p.place[key];
+  const uint32_t owner = __ldcg(p.owner + key);
+  const int64_t place = __ldcg(p.place + key);
   // An entry that overlaps another page without being it cannot move.
   const bool same = owner == (uint32_t)e || ((p.table[owner] ^ d) & ~(int64_t)0xfc) == 0;
   if (threadIdx.x == 0) {
@@ -208,7 +275,7 @@ __global__ void __launch_bounds__(kCopyThreads) compact_move_kernel(const Compac
     p.out[e] = !same || place < 0 ? 0 : (place << 8) | (d & 255);
   }
   if (owner != (uint32_t)e || place < 0) return;
-  copy_units(p.arena + desc_offset(d), p.into + place, 0, p.bytes(desc_mode(d)) / 16);
+  copy_units<4>(p.arena + desc_offset(d), p.into + place, 0, (int)(p.bytes(desc_mode(d)) / 16));
 }
 
 static int check_page_geometry(int heads, int head_dim, int group) {
@@ -253,12 +320,17 @@ extern "C" int akv_fork_pages(const int64_t *table, int64_t layer_stride, int64_
   if (rows == 0 || columns == 0) return AKV_OK;
   const int64_t span = (layers - 1) * layer_stride + (int64_t)(batch - 1) * seq_stride + columns;
   if (overlap(table, 8 * span, out_table, 8 * rows * columns)) return AKV_ERR_INVALID;
-  const int parts = std::max(1, std::min(heads, 8));  // 8 KB of an 8-head FP16 page of head_dim 128 a CTA
+  // A page is cut into 32 KB parts; finer, down to 8 KB, where the rows alone do not
+  // fill the device.
+  const int64_t page = page_bytes(heads, head_dim, group)(AKV_MODE_FP16);
+  const int64_t most = std::max<int64_t>(1, page >> 13), least = std::max<int64_t>(1, page >> 15);
+  const int parts = (int)std::max(least, std::min(most, 8 * 148 / rows));
   if (rows * parts >= (1ll << 31)) return AKV_ERR_UNSUPPORTED;
   const ForkParams p{table, layer_stride, seq_stride, batch, children, columns, uniform_tokens, parts, tokens, parents,
                      fresh, out_table, (uint8_t *)arena, arena_bytes, page_bytes(heads, head_dim, group), dev_status};
-  fork_pages_kernel<<<(unsigned)(rows * parts), kCopyThreads, 0, (cudaStream_t)stream>>>(p);
-  return cudaGetLastError() == cudaSuccess ? AKV_OK : AKV_ERR_CUDA;
+  const cudaError_t err =
+      launch_dependent(fork_pages_kernel, (unsigned)(rows * parts), kCopyThreads, 0, (cudaStream_t)stream, p);
+  return err == cudaSuccess ? AKV_OK : AKV_ERR_CUDA;
 }
 
 extern "C" int64_t akv_compact_workspace_bytes(int64_t entries, int64_t arena_bytes, int heads, int head_dim,
@@ -298,10 +370,15 @@ extern "C" int akv_compact_pages(const int64_t *table, int64_t entries, int64_t 
   p.counts = (int32_t *)(ws + z.counts_at), p.blocks = (int32_t)z.blocks;
   p.status = dev_status;
   cudaStream_t s = (cudaStream_t)stream;
-  if (cudaMemsetAsync(p.owner, 0xff, 4 * z.keys, s) != cudaSuccess) return AKV_ERR_CUDA;
-  compact_mark_kernel<<<(unsigned)std::min<int64_t>((entries + 255) / 256, 4 * 148), 256, 0, s>>>(p);
-  compact_count_kernel<<<(unsigned)z.blocks, kRankThreads, 0, s>>>(p);
-  compact_rank_kernel<<<(unsigned)z.blocks, kRankThreads, 0, s>>>(p);
-  compact_move_kernel<<<(unsigned)entries, kCopyThreads, 0, s>>>(p);
-  return cudaGetLastError() == cudaSuccess ? AKV_OK : AKV_ERR_CUDA;
+  cudaError_t err;
+  if (entries <= kOnePlan && z.keys <= 8 * kOnePlan) {
+    err = launch_dependent(compact_plan_kernel, 1, kRankThreads, 0, s, p, (int)z.keys);
+  } else {
+    if (cudaMemsetAsync(p.owner, 0xff, 4 * z.keys, s) != cudaSuccess) return AKV_ERR_CUDA;
+    compact_mark_kernel<<<(unsigned)std::min<int64_t>((entries + 255) / 256, 4 * 148), 256, 0, s>>>(p);
+    err = launch_dependent(compact_count_kernel, (unsigned)z.blocks, kRankThreads, 0, s, p);
+    if (err == cudaSuccess) err = launch_dependent(compact_rank_kernel, (unsigned)z.blocks, kRankThreads, 0, s, p);
+  }
+  if (err == cudaSuccess) err = launch_dependent(compact_move_kernel, (unsigned)entries, kCopyThreads, 0, s, p);
+  return err == cudaSuccess ? AKV_OK : AKV_ERR_CUDA;
 }
