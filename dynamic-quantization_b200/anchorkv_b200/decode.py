@@ -169,7 +169,7 @@ def packed_attention(query, layer, scale, splits=4, *, out=None, window=None, si
                             or out.device != query.device or out.stride(-1) != 1):
         raise ValueError("out must be an FP16 tensor of the query's shape on its device, unit stride in head_dim")
     if query.stride(-1) != 1 or query.stride(1) % 8 or query.stride(0) % 8 or query.data_ptr() % 16:
-        query = query.contiguous()
+        query = query.clone(memory_format=torch.contiguous_format)  # contiguous() keeps an odd address
     arena, arena_bytes, table, seq_blocks, max_blocks = _store_geometry(layer)
     if out is None:
         out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
@@ -222,6 +222,8 @@ def _by_position(query, layer, scale, splits, window, sinks, out):
     table = layer.table if batched else layer.table.view(1, -1)
     if pool.arena.device != dev or table.device != dev:
         raise ValueError("the query and the pages must be on one device")
+    if table.dtype != torch.int64 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError("the page table must be an int64 tensor [batch, max_blocks], unit stride in max_blocks")
     seq_blocks = layer.seq_blocks if batched else None
     max_blocks = layer.max_blocks if batched else len(layer.pages)
     tokens, uniform = _layer_tokens(layer, batched, batch, dev)
@@ -229,7 +231,7 @@ def _by_position(query, layer, scale, splits, window, sinks, out):
         return out
     qb, qh, qt, qd = query.stride()
     if qd != 1 or (qb | qh | qt) & 7 or query.data_ptr() & 15:
-        query = query.contiguous()
+        query = query.clone(memory_format=torch.contiguous_format)  # contiguous() keeps an odd address
         qb, qh, qt, _ = query.stride()
     width = 0 if window is None else min(window, 1 << 30)
     sinks = min(sinks, 1 << 30)
@@ -242,7 +244,7 @@ def _by_position(query, layer, scale, splits, window, sinks, out):
         ws = _workspace(dev, nbytes, stream)
         _lib.call("akv_chunk_attention", pool.arena.data_ptr(), pool.nbytes, table.data_ptr(), table.stride(0),
                   None if seq_blocks is None else seq_blocks.data_ptr(), max_blocks, tokens, uniform,
-                  query.data_ptr(), qb, qh, qt, batch, rows, heads, pool.heads, dim, pool.group, scale, width, sinks,
+                  query.data_ptr(), qb, qh, qt, batch, rows, heads, pool.heads, dim, pool.group, float(scale), width, sinks,
                   splits, out.data_ptr(), ob, oh, ot, ws.data_ptr(), ws.numel(), _lib.status_ptr(dev), stream)
     return out
 

@@ -321,7 +321,7 @@ class PagedKVStore:
     def bits(self, layer: int = 0) -> np.ndarray:
         """Precision of every page, ``[batch, pages]``."""
         modes = self._desc[layer, :, :self.pages(layer)] & 3
-        return np.vectorize(P.MODE_TO_BITS.get)(modes)
+        return np.vectorize(P.MODE_TO_BITS.get, otypes=[np.int64])(modes)
 
     @property
     def payload_bytes(self) -> int:
@@ -348,9 +348,10 @@ class PagedKVStore:
         desc = self.tables[layer, :, :n].contiguous()
         k = torch.empty((self.heads, self.batch * n * P.BLOCK, self.dim), dtype=torch.float16, device=self.device)
         v = torch.empty_like(k)
-        _lib.call("akv_unpack_pages", desc.data_ptr(), self.batch * n, self.pool.arena.data_ptr(), self.pool.nbytes,
-                  self.heads, self.dim, self.group, k.data_ptr(), v.data_ptr(), _lib.DTYPE_F16,
-                  _lib.status_ptr(self.device), _lib.stream_of(self.device))
+        if n:
+            _lib.call("akv_unpack_pages", desc.data_ptr(), self.batch * n, self.pool.arena.data_ptr(),
+                      self.pool.nbytes, self.heads, self.dim, self.group, k.data_ptr(), v.data_ptr(), _lib.DTYPE_F16,
+                      _lib.status_ptr(self.device), _lib.stream_of(self.device))
         shape = (self.heads, self.batch, n * P.BLOCK, self.dim)
         length = self.lengths[layer]
         return (k.view(shape).transpose(0, 1)[:, :, :length], v.view(shape).transpose(0, 1)[:, :, :length])
@@ -463,9 +464,13 @@ def paged_route(model, cache, backend: str = "packed"):
 
 
 def decode_step(model, cache, tokens: torch.Tensor):
-    """One batched decode step: ``tokens`` ``[batch]`` -> last-position logits ``[batch, vocab]``."""
+    """One batched step.  ``tokens`` ``[batch]`` or ``[batch, 1]`` (a decoded token
+    per sequence) gives last-position logits ``[batch, vocab]``; ``[batch, n]`` (a
+    prompt's next chunk, or drafted tokens to verify) logits ``[batch, n, vocab]``."""
     position = cache.get_seq_length()
-    out = model(input_ids=tokens.view(-1, 1), past_key_values=cache,
-                cache_position=torch.tensor([position], device=tokens.device),
-                attention_mask={"full_attention": None}, use_cache=True, logits_to_keep=1)
-    return out.logits[:, -1]
+    rows = tokens.shape[1] if tokens.dim() == 2 else 1
+    out = model(input_ids=tokens.reshape(-1, rows), past_key_values=cache,
+                cache_position=torch.arange(position, position + rows, device=tokens.device),
+                attention_mask={"full_attention": None, "sliding_attention": None}, use_cache=True,
+                logits_to_keep=rows)
+    return out.logits if rows > 1 else out.logits[:, -1]

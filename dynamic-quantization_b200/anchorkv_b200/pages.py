@@ -111,6 +111,11 @@ def compact_pages(pool: PagePool, table: torch.Tensor, into: PagePool, live: dic
         into.check_free(b, n)
     flat = table.contiguous()
     dev = table.device
+    source, target = pool.arena.data_ptr(), into.arena.data_ptr()
+    if source < target + into.nbytes and target < source + pool.nbytes:
+        raise ValueError("the target pool must have an arena of its own")
+    if flat.numel() == 0:
+        return flat.clone()
     with _lib.on_device(dev):
         nbytes = _lib.load().akv_compact_workspace_bytes(flat.numel(), pool.nbytes, pool.heads, pool.dim, pool.group)
         if nbytes < 0:

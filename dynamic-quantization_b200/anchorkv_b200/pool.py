@@ -245,8 +245,9 @@ class PagePool:
         never grows: a request for more slots raises MemoryError."""
         if dim not in (64, 128) or not group_ok(dim, group):
             raise ValueError(f"supported geometry: head dim 64 or 128, scale groups 32, 64, 128, {BLOCK * dim}")
-        if arena.dtype != torch.uint8 or arena.dim() != 1 or not arena.is_contiguous() or arena.data_ptr() % 16:
-            raise ValueError("the arena must be a contiguous, 16-byte aligned one-dimensional uint8 tensor")
+        if arena.dtype != torch.uint8 or arena.dim() != 1 or not arena.is_contiguous() or arena.data_ptr() % 16 \
+                or not arena.is_cuda:
+            raise ValueError("the arena must be a contiguous, 16-byte aligned one-dimensional uint8 CUDA tensor")
         pool = cls.__new__(cls)
         pool.device, pool.fixed = arena.device, True
         pool._lay_out(heads, dim, group, pages)

@@ -200,7 +200,7 @@ __device__ __forceinline__ ChunkView chunk_view(const ChunkParams &p, int b, int
   const ChunkArgs &a = p.a;
   ChunkView v;
   const int held = a.seq_blocks ? max(0, min(__ldg(a.seq_blocks + b), a.columns)) : a.columns;
-  const int tokens = min(a.tokens ? __ldg(a.tokens + b) : a.uniform_tokens, kBlock * held);
+  const int tokens = max(0, min(a.tokens ? __ldg(a.tokens + b) : a.uniform_tokens, kBlock * held));
   v.at_first = tokens - a.rows;
   v.row0 = row0, v.n = nrows;
   v.at_lo = v.at_first + fdiv(row0, p.fd_hpk);
@@ -500,28 +500,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-// Of every 16 pairs of weights, this many are worked out on the FMA pipe
-// (exp2_poly), the rest by ex2: the special-function unit takes one result a lane
-// and four clocks, and alone would take longer than the MMAs of a tile.
-constexpr int kPolyPairs = 0;
-// 2^x for two finite or -inf x <= 9: x = n + f with n whole and |f| <= 1/2 (adding
-// and taking away 1.5 * 2^23 rounds to whole numbers), 2^f by the degree-4
-// polynomial of least largest relative error on that range (2.6e-6, found with
-// Remez's exchange; the rounding to fp16 that follows is 2^-11), and n added to the
-// exponent bits.  Below 2^-126 it stays there: such a weight is 0 in fp16.
-__device__ __forceinline__ uint64_t exp2_poly(uint64_t x) {
-  auto twice = [](float v) { return f2_pack(v, v); };
-  x = f2_pack(fmaxf(f2_lo(x), -126.f), fmaxf(f2_hi(x), -126.f));
-  const uint64_t t = f2_add(x, twice(12582912.f));
-  const uint64_t f = f2_sub(x, f2_sub(t, twice(12582912.f)));
-  uint64_t p = f2_fma(twice(0.009570102207362652f), f, twice(0.05591785907745361f));
-  p = f2_fma(p, f, twice(0.240247443318367f));
-  p = f2_fma(p, f, twice(0.6931217908859253f));
-  p = f2_fma(p, f, twice(0.9999992847442627f));
-  const uint32_t lo = ((uint32_t)t << 23) + (uint32_t)p, hi = ((uint32_t)(t >> 32) << 23) + (uint32_t)(p >> 32);
-  return (uint64_t)lo | ((uint64_t)hi << 32);
-}
-
 // 32 normalised outputs of a row.
 __device__ __forceinline__ void store_out32(__half *out, const float (&o)[32], float inv, bool vector) {
   uint32_t w[16];
@@ -646,7 +624,7 @@ __device__ __forceinline__ void chunk_softmax(const TileWork &work, ChunkShared<
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const uint64_t x2 = f2_fma(f2_pack(s[16 * i + 2 * k], s[16 * i + 2 * k + 1]), c2, neg2);
-            const uint64_t p2 = k < kPolyPairs ? exp2_poly(x2) : f2_pack(ex2(f2_lo(x2)), ex2(f2_hi(x2)));
+            const uint64_t p2 = f2_pack(ex2(f2_lo(x2)), ex2(f2_hi(x2)));
             sum[k & 1] = f2_add(sum[k & 1], p2);
             pk[k] = pack_f16x2(f2_lo(p2), f2_hi(p2));
           }
@@ -930,44 +908,43 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(const __grid_constant_
   if (cut.w == 0 || r >= p.rows_kv - row0) return;
   int c1 = c0 + 1;
   while (c1 < p.ctas - 1 && __ldcg(&p.w.cuts[c1].x) == 1) ++c1;
-  {
-    float m = -INFINITY, l = 0.f, acc[VEC];
+  float m = -INFINITY, l = 0.f, acc[VEC];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
-    constexpr int CB = 4;  // shares whose loads are in flight together
-    for (int c = c0; c <= c1; c += CB) {
-      float2 ml[CB];
-      float o[CB][VEC];
+  for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
+  constexpr int CB = 4;  // shares whose loads are in flight together
+  for (int c = c0; c <= c1; c += CB) {
+    float2 ml[CB];
+    float o[CB][VEC];
 #pragma unroll
-      for (int j = 0; j < CB; ++j) {
-        ml[j].x = -INFINITY;
-        if (c + j <= c1) {
-          const float *part = p.partials + ((2ll * (c + j) + (c + j == c0 ? 1 : 0)) * 256 + r) * kRowStride;
-          ml[j] = __ldcg(reinterpret_cast<const float2 *>(part + D));
+    for (int j = 0; j < CB; ++j) {
+      ml[j].x = -INFINITY;
+      if (c + j <= c1) {
+        const float *part = p.partials + ((2ll * (c + j) + (c + j == c0 ? 1 : 0)) * 256 + r) * kRowStride;
+        ml[j] = __ldcg(reinterpret_cast<const float2 *>(part + D));
 #pragma unroll
-          for (int i = 0; i < VEC; i += 2) {
-            const float2 v = __ldcg(reinterpret_cast<const float2 *>(part + VEC * lane + i));
-            o[j][i] = v.x, o[j][i + 1] = v.y;
-          }
+        for (int i = 0; i < VEC; i += 2) {
+          const float2 v = __ldcg(reinterpret_cast<const float2 *>(part + VEC * lane + i));
+          o[j][i] = v.x, o[j][i + 1] = v.y;
         }
       }
-#pragma unroll
-      for (int j = 0; j < CB; ++j) {
-        if (ml[j].x == -INFINITY) continue;
-        const float top = fmaxf(m, ml[j].x), x = ex2(m - top), y = ex2(ml[j].x - top);
-        l = l * x + ml[j].y * y;
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) acc[i] = acc[i] * x + o[j][i] * y;
-        m = isnan(ml[j].x) ? ml[j].x : top;
-      }
     }
-    const int rho = row0 + r, tok = fdiv(rho, p.fd_hpk), h = kvh * p.heads_per_kv + (rho - tok * p.heads_per_kv);
-    __half *out = a.out + (int64_t)b * a.o_bs + (int64_t)h * a.o_hs + (int64_t)tok * a.o_ts + VEC * lane;
-    const float inv = l > 0.f ? 1.f / l : l;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) out[i] = __float2half_rn(acc[i] * inv);
+    for (int j = 0; j < CB; ++j) {
+      if (ml[j].x == -INFINITY) continue;
+      const float top = fmaxf(m, ml[j].x), x = ex2(m - top), y = ex2(ml[j].x - top);
+      l = l * x + ml[j].y * y;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) acc[i] = acc[i] * x + o[j][i] * y;
+      m = isnan(ml[j].x) ? ml[j].x : top;
+    }
   }
+  const int rho = row0 + r, tok = fdiv(rho, p.fd_hpk), h = kvh * p.heads_per_kv + (rho - tok * p.heads_per_kv);
+  __half *out = a.out + (int64_t)b * a.o_bs + (int64_t)h * a.o_hs + (int64_t)tok * a.o_ts + VEC * lane;
+  const float inv = l > 0.f ? 1.f / l : l;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) out[i] = __float2half_rn(acc[i] * inv);
 }
+
 // ------------------------------------------------------------------- host
 // SMs of the current device (one CTA each), 0 on error.
 static int device_sms() {
@@ -1005,7 +982,7 @@ static cudaError_t launch_tiles(const ChunkParams &p) {
   if (cudaError_t err = launch_dependent(chunk_plan_kernel, p.a.batch, 1024, 0, s, p)) return err;
   // 16 KV-head-pages a warp where there are tiles enough for the device, down to one
   const int64_t tiles = (int64_t)p.w.tiles_max * p.a.batch;
-  const int jobs = 2 * kTilePages * p.a.kv_heads / 8;  // of a tile, per warp of a CTA
+  const int jobs = std::min(2 * kTilePages * p.a.kv_heads / 8, 65535);  // of a tile, per warp of a CTA
   const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(jobs, std::max<int64_t>(jobs / 16, 8 * p.ctas / std::max<int64_t>(tiles, 1))));
   if (p.w.tiles_max > 0)
     if (cudaError_t err =
@@ -1057,14 +1034,24 @@ static ChunkArgs slice_of(ChunkArgs a, int first, int count) {
   return a;
 }
 static int slice_batch(const ChunkArgs &a, int sms) {
-  ChunkArgs one = a;
-  one.batch = 1;
-  return (int)std::max<int64_t>(1, std::min<int64_t>(a.batch, kSpaceBytes / chunk_layout(one, sms, nullptr, nullptr)));
+  ChunkArgs some = a;
+  some.batch = 1;
+  const int64_t one = chunk_layout(some, sms, nullptr, nullptr);
+  some.batch = 2;
+  const int64_t each = std::max<int64_t>(1, chunk_layout(some, sms, nullptr, nullptr) - one);  // the rest is shared
+  const int64_t fit = 1 + std::max<int64_t>(0, kSpaceBytes - one) / each;
+  return (int)std::min<int64_t>({fit, a.batch, 65535});  // a grid's second dimension
+}
+
+// Tiles of a KV head's row blocks are counted in 32 bits.
+static bool countable(const ChunkArgs &a) {
+  const int64_t blocks = ((int64_t)a.rows * (a.q_heads / a.kv_heads) + 255) / 256;
+  return blocks * (a.columns / kTilePages + 2) < (1ll << 31);
 }
 
 int64_t chunk_tiles_bytes(const ChunkArgs &a) {
   const int sms = device_sms();
-  if (sms <= 0) return -1;
+  if (sms <= 0 || !countable(a)) return -1;
   ChunkArgs part = a;
   part.batch = slice_batch(a, sms);
   return chunk_layout(part, sms, nullptr, nullptr);
@@ -1073,6 +1060,7 @@ int64_t chunk_tiles_bytes(const ChunkArgs &a) {
 int chunk_tiles_launch(const ChunkArgs &all, void *workspace, int64_t workspace_bytes) {
   const int sms = device_sms();
   if (sms <= 0) return AKV_ERR_CUDA;
+  if (!countable(all)) return AKV_ERR_UNSUPPORTED;
   if (workspace_bytes < chunk_tiles_bytes(all)) return AKV_ERR_INVALID;
   const int step = slice_batch(all, sms);
   for (int first = 0; first < all.batch; first += step) {

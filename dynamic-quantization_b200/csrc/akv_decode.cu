@@ -407,7 +407,7 @@ __device__ __forceinline__ ItemRows item_rows(const DecodeParams &p, int item) {
   ItemRows v;
   const int b = fdiv(item, p.fd_ipb);
   v.held = p.seq_blocks ? max(0, min(__ldg(p.seq_blocks + b), p.columns)) : p.columns;
-  const int tokens = min(p.tokens ? __ldg(p.tokens + b) : p.uniform_tokens, kBlock * v.held);
+  const int tokens = max(0, min(p.tokens ? __ldg(p.tokens + b) : p.uniform_tokens, kBlock * v.held));
   v.at_first = tokens - p.rows;
   v.row0 = 8 * (item - fdiv(item, p.fd_qgroups) * p.qgroups);  // items are kv_heads * qgroups per sequence
   v.n = min(8, p.gqa - v.row0);
@@ -1474,7 +1474,7 @@ static int decode_launch(const void *arena, int64_t arena_bytes, const int64_t *
                          void *workspace, int64_t workspace_bytes, int32_t *dev_status, cudaStream_t s,
                          const RowsArgs *rows = nullptr) {
   if (!arena || !table || !query || !workspace) return AKV_ERR_INVALID;
-  if (table_stride < (rows ? rows->columns : max_blocks) || arena_bytes < 0 || !isfinite(scale)) return AKV_ERR_INVALID;
+  if (table_stride < max_blocks || arena_bytes < 0 || !isfinite(scale)) return AKV_ERR_INVALID;
   if (((uintptr_t)arena & 15) || ((uintptr_t)query & 15) || ((uintptr_t)workspace & 15))
     return AKV_ERR_INVALID;
   if (q_batch_stride % 8 || q_head_stride % 8) return AKV_ERR_INVALID;
@@ -1761,7 +1761,10 @@ extern "C" int akv_chunk_attention(const void *arena, int64_t arena_bytes, const
                                    int32_t window, int32_t sinks, int32_t splits, void *out, int64_t out_batch_stride,
                                    int64_t out_head_stride, int64_t out_token_stride, void *workspace,
                                    int64_t workspace_bytes, int32_t *dev_status, void *stream) {
-  if (!out || q_token_stride % 8 || (!tokens && uniform_tokens < 0)) return AKV_ERR_INVALID;
+  if (!arena || !table || !query || !out || !workspace || arena_bytes < 0 || !isfinite(scale)) return AKV_ERR_INVALID;
+  if (((uintptr_t)arena & 15) || ((uintptr_t)query & 15) || ((uintptr_t)workspace & 15)) return AKV_ERR_INVALID;
+  if (q_batch_stride % 8 || q_head_stride % 8 || q_token_stride % 8) return AKV_ERR_INVALID;
+  if (table_stride < max_blocks || (!tokens && uniform_tokens < 0)) return AKV_ERR_INVALID;
   ChunkPlan c;
   if (int st = chunk_plan(batch, rows, q_heads, kv_heads, head_dim, max_blocks, window, sinks, &c)) return st;
   if (group != 32 && group != 64 && group != 128 && group != 16 * head_dim) return AKV_ERR_UNSUPPORTED;
@@ -1770,16 +1773,13 @@ extern "C" int akv_chunk_attention(const void *arena, int64_t arena_bytes, const
   c.rows.q_ts = q_token_stride;
   cudaStream_t s = (cudaStream_t)stream;
   if (use_tiles(c, batch, kv_heads)) {
-    if (!arena || !table || !query || !workspace || ((uintptr_t)workspace & 15) || table_stride < max_blocks || arena_bytes < 0 || !isfinite(scale)) return AKV_ERR_INVALID;
-    if (((uintptr_t)arena & 15) || ((uintptr_t)query & 15) || q_batch_stride % 8 || q_head_stride % 8) return AKV_ERR_INVALID;
-    const int lg = ilog2_exact(group);
     ChunkArgs a = {};
     a.arena = (const uint8_t *)arena, a.arena_bytes = arena_bytes, a.table = table, a.table_stride = table_stride;
     a.seq_blocks = seq_blocks, a.columns = max_blocks, a.tokens = tokens, a.uniform_tokens = c.rows.uniform_tokens;
     a.q = (const __half *)query, a.q_bs = q_batch_stride, a.q_hs = q_head_stride, a.q_ts = q_token_stride;
     a.out = (__half *)out, a.o_bs = out_batch_stride, a.o_hs = out_head_stride, a.o_ts = out_token_stride;
     a.batch = batch, a.rows = rows, a.q_heads = q_heads, a.kv_heads = kv_heads, a.head_dim = head_dim;
-    a.log2_group = lg, a.window = c.rows.window, a.sinks = c.rows.sinks, a.lead = c.rows.lead;
+    a.log2_group = ilog2_exact(group), a.window = c.rows.window, a.sinks = c.rows.sinks, a.lead = c.rows.lead;
     a.scale = scale, a.status = dev_status, a.stream = s;
     return chunk_tiles_launch(a, workspace, workspace_bytes);
   }

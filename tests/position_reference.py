@@ -58,3 +58,28 @@ def assert_rows_close(actual, expected, tolerance):
     assert np.isfinite(a).all()
     worst = np.unravel_index(np.argmax(over), over.shape)
     assert over.max() <= 0, f"at {worst}: {a[worst]} against {expected[worst]}, tolerance {tolerance[worst]:.3g}"
+
+
+def attention_rows_torch(q, k, v, held, tokens, scale, window=None, sinks=0):
+    """attention_rows_f64 of one sequence as float64 matrix products on the tensors' device, for long ones.
+
+    ``q``: ``[Hq, R, D]``; ``k``, ``v``: ``[Hkv, T, D]``; ``held``: ``[T]`` bool; gives numpy arrays ``[Hq, R, D]``."""
+    import torch
+
+    groups = q.shape[0] // k.shape[0]
+    q, k, v = q.double(), k.double().repeat_interleave(groups, 0), v.double().repeat_interleave(groups, 0)
+    rows, span = q.shape[1], k.shape[1]
+    at = torch.arange(tokens - rows, tokens, device=q.device)[:, None]
+    pos = torch.arange(span, device=q.device)
+    seen = held & (pos <= at) & (pos < tokens) & (at >= 0)
+    if window is not None:
+        seen = seen & ((pos > at - window) | (pos < sinks))
+    s = (q @ k.transpose(1, 2) * scale).masked_fill(~seen, -torch.inf)
+    w = torch.exp(s - s.amax(-1, keepdim=True).clamp_min(-1e300)) * seen
+    w = w / w.sum(-1, keepdim=True).clamp_min(1e-300)
+    o = w @ v
+    some = seen.any(-1)[None, :, None]
+    largest = v.abs().amax((1, 2))[:, None, None]
+    tol = ((2.0 ** -11 + 2.0 ** -13) * (w @ v.abs()) + 2.0 ** -11 * o.abs()
+           + seen.sum(-1)[None, :, None] * 2.0 ** -25 * largest + 2.0 ** -25) * some
+    return o.cpu().numpy(), tol.cpu().numpy()
