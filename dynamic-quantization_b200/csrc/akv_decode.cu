@@ -1728,12 +1728,16 @@ static int chunk_plan(int batch, int rows, int q_heads, int kv_heads, int head_d
 }
 // Whether a chunk runs on tcgen05 tiles (akv_chunk.cu) or on the stream-K decode.
 // The decode dequantises every page once per 8 rows of its KV head; the tiles
-// unpack it once and then share it among 256 rows, but need four launches.  Measured
-// on a B200 with P pages x KV heads and g groups of 8 rows: the decode 15 us +
-// 0.85 ns P g, the tiles 45 us + (2.2 + 0.06 g) ns P.
+// unpack it once, write and read it as fp16, and then share it among 256 rows, in
+// four launches.  Measured on a B200, head_dim 128, 2 query heads a KV head, P pages
+// x KV heads and g groups of 8 rows, decode against tiles in us:
+//   P 2048    INT4  g 16: 44, 54    g 32: 63, 65     FP16  g 16: 55, 53    g 32: 83, 63
+//   P 16384   INT4  g 8: 100, 122   g 12: 136, 125   FP16  g 6: 128, 115   g 8: 161, 118
+//   P 65536   INT4  g 8: 321, 340   g 12: 470, 345   FP16  g 4: 359, 318   g 8: 668, 322
+// The host does not know the pages' precisions, so the border lies between theirs.
 static bool use_tiles(const ChunkPlan &c, int batch, int kv_heads) {
   const int64_t pages = (int64_t)batch * kv_heads * c.columns, groups = (c.rows_total / kv_heads + 7) / 8;
-  return pages * (groups - 4) > 40000;
+  return pages * (groups - 6) > 40000;
 }
 }  // namespace akv
 

@@ -13,7 +13,7 @@ from position_reference import assert_rows_close, attention_rows_torch
 pytestmark = pytest.mark.gpu
 
 # rows, tokens: a chunk that runs on the decode, and one on the operand tiles
-SMALL, LARGE = (5, [150, 70]), (300, [2500, 450])
+SMALL, LARGE = (5, [150, 70]), (2100, [2500, 2150])
 SIZES = pytest.mark.parametrize("rows,lengths", [SMALL, LARGE], ids=["decode", "tiles"])
 HQ, HKV = 16, 2
 
@@ -248,7 +248,7 @@ def test_python_refusals(cuda):
 
 
 @pytest.mark.parametrize("dim", [64, 128])
-@pytest.mark.parametrize("columns", [250, 999, 1000, 1001, 1002, 1003, 4000])
+@pytest.mark.parametrize("columns", [250, 1000, 1051, 1052, 1053, 1054, 4000])
 def test_a_long_sequence_with_many_rows(cuda, dim, columns):
     """Both ways of running a chunk, over lengths around where one takes over."""
     n = 16 * columns - 7
