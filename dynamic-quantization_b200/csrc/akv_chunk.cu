@@ -5,7 +5,7 @@
 // 128 tokens (8 resident pages; evicted pages take no place in a tile):
 //
 //   S = Q K^T          tcgen05.mma, both operands in shared memory, S in TMEM
-//   P = 2^(c S - m)    one thread per row: running max m and sum l in fp32
+//   P = 2^(c S - m)    two threads per row: running max m and sum l in fp32
 //   O = O + P V        tcgen05.mma, P (fp16) in TMEM over S's columns, O in TMEM
 //
 // P is rounded to fp16 because the MMA takes both operands in one 16-bit type and
@@ -18,6 +18,20 @@
 // share every K and V tile; the work (row tiles x tiles of tokens) is cut into equal
 // contiguous ranges, one per CTA, whose partial (O, m, l) a merge kernel joins.
 // Waits are bounded: a role whose wait runs out reports AKV_DEV_TIMEOUT and leaves.
+//
+// What bounds it, measured on a B200 with clocks read in the kernel: a tile of tokens
+// takes about 3500 to 3700 clocks.  Of these a row tile's warps spend 150 on reading S,
+// 250 on the max, 200 on agreeing on it, 1350 on the exponentials (1024 if the
+// special-function unit did nothing else) and 150 on handing P over; its next S is
+// there 1300 (head_dim 64) to 1700 clocks (128) later, behind O += P V, while the other
+// row tile is at its exponentials.  A 2048-token chunk of 32768 (32 heads over 8, 128)
+// takes 905 us, 1.1 PFLOP/s; 1000 tokens through a window of
+// 2048 (4 sequences, 24 heads over 8, 64) 154 us, of which the tiles take 115.
+// Slower or no faster were: tiles of 64 tokens with S twice; S a tile ahead of P where
+// head_dim 64 leaves TMEM for it (149 to 157 us against 154); a thread per row tile
+// issuing the MMAs (1296 against 905); exponentials of some pairs by a polynomial
+// (993 against 963 for one of 16); weights tried against the old max before a new one
+// is looked for (171 against 154); one thread a row.
 #include <math.h>
 #include <stddef.h>
 
@@ -447,15 +461,13 @@ __device__ __forceinline__ void chunk_mma(const TileWork &work, ChunkShared<D> &
       const bool last = sh.meta[metas++ % Shared::kMetas].last;
       const int v_fill = mma.n++;
       if (!last) k_fill = mma.n++;
-      ok = mma.filled(v_fill);
+      ok = mma.filled(v_fill) && (last || mma.filled(k_fill));  // before the weights, not behind them
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         if (!ok || x >= streams) break;
         ok = mma.values(x, v_fill, !first);
         if (x == streams - 1) mma.release(v_fill);
         if (!ok || last) continue;
-        if (x == 0) ok = mma.filled(k_fill);
-        if (!ok) break;
         mma.scores(x, x, k_fill);
         if (x == streams - 1) mma.release(k_fill);
       }
