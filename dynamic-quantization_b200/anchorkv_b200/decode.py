@@ -90,6 +90,8 @@ def _store_geometry(layer):
 
 def _as_table(layer):
     """A DeclarativeKVCache stands for its (single) layer's visible page table."""
+    if isinstance(layer, PagedBatch):
+        return layer
     if hasattr(layer, "decode_view"):
         if layer.layers > 1:
             raise ValueError("the store holds several layers: pass store.decode_view(layer)")
@@ -128,14 +130,15 @@ def _check_query(query, layer, splits, *, empty_ok: bool) -> int:
     LSE merge); an output needs at least one page, as in the reference."""
     batched = isinstance(layer, PagedBatch)
     batch = layer.batch if batched else 1
-    if query.dim() != 4 or query.shape[0] != batch or query.shape[2] != 1 or query.shape[-1] != layer.dim:
+    shape = query.shape
+    if len(shape) != 4 or shape[0] != batch or shape[2] != 1 or shape[3] != layer.dim:
         raise ValueError('packed kernel supports batch=1, query length=1 only' if not batched
                          else 'query must be [batch, heads, 1, head_dim] for the page table')
     length = layer.max_blocks if batched else layer.length
     if query.dtype != torch.float16 or not query.is_cuda or (length == 0 and not empty_ok):
         raise ValueError('packed kernel requires a nonempty CUDA FP16 cache')
     _check_layout(layer)
-    if query.shape[1] % layer.heads:
+    if shape[1] % layer.heads:
         raise ValueError('query heads must be divisible by KV heads')
     if splits < 0:
         raise ValueError('splits must be non-negative')
@@ -194,9 +197,8 @@ def _check_window(window, sinks) -> None:
         raise ValueError("sinks must be non-negative and come with a window")
 
 
-def _layer_tokens(layer, batched, batch, device):
+def _token_counts(tokens, batch, device):
     """(device address or None, uniform count) of the tokens each sequence holds."""
-    tokens = layer.tokens if batched else layer.length
     if tokens is None:
         raise ValueError("the page table has no token counts (PagedBatch.over(pool, table, tokens=...)), so its "
                          "columns have no positions")
@@ -214,19 +216,21 @@ def _by_position(query, layer, scale, splits, window, sinks, out):
     shape, dev = query.shape, query.device
     batch, heads, rows, dim = shape
     if out is None:
-        out = torch.empty(shape, dtype=torch.float16, device=dev)
+        out = query.new_empty(shape)
     elif out.dtype != torch.float16 or out.shape != shape or out.device != dev or out.stride(-1) != 1:
         raise ValueError("out must be an FP16 tensor of the query's shape on its device, unit stride in head_dim")
-    batched = isinstance(layer, PagedBatch)
     pool = layer.pool
-    table = layer.table if batched else layer.table.view(1, -1)
-    if pool.arena.device != dev or table.device != dev:
+    arena, page_heads = pool.arena, pool.heads
+    if isinstance(layer, PagedBatch):
+        table, seq_blocks, max_blocks, tokens = layer.table, layer.seq_blocks, layer.max_blocks, layer.tokens
+    else:
+        table, seq_blocks, max_blocks, tokens = layer.table.view(1, -1), None, len(layer.pages), layer.length
+    if arena.device != dev or table.device != dev:
         raise ValueError("the query and the pages must be on one device")
-    if table.dtype != torch.int64 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
+    table_stride = table.stride()
+    if table.dtype != torch.int64 or len(table_stride) != 2 or (max_blocks > 1 and table_stride[1] != 1):
         raise ValueError("the page table must be an int64 tensor [batch, max_blocks], unit stride in max_blocks")
-    seq_blocks = layer.seq_blocks if batched else None
-    max_blocks = layer.max_blocks if batched else len(layer.pages)
-    tokens, uniform = _layer_tokens(layer, batched, batch, dev)
+    tokens, uniform = _token_counts(tokens, batch, dev)
     if rows == 0 or heads == 0 or batch == 0:
         return out
     qb, qh, qt, qd = query.stride()
@@ -237,14 +241,14 @@ def _by_position(query, layer, scale, splits, window, sinks, out):
     sinks = min(sinks, 1 << 30)
     ob, oh, ot, _ = out.stride()
     with _lib.on_device(dev):
-        nbytes = _chunk_bytes(dev, batch, rows, heads, pool.heads, dim, max_blocks, width, sinks, splits)
+        nbytes = _chunk_bytes(dev, batch, rows, heads, page_heads, dim, max_blocks, width, sinks, splits)
         if nbytes < 0:
             raise ValueError('unsupported decode geometry')
         stream = _lib.stream_of(dev)
         ws = _workspace(dev, nbytes, stream)
-        _lib.call("akv_chunk_attention", pool.arena.data_ptr(), pool.nbytes, table.data_ptr(), table.stride(0),
+        _lib.call("akv_chunk_attention", arena.data_ptr(), pool.nbytes, table.data_ptr(), table_stride[0],
                   None if seq_blocks is None else seq_blocks.data_ptr(), max_blocks, tokens, uniform,
-                  query.data_ptr(), qb, qh, qt, batch, rows, heads, pool.heads, dim, pool.group, float(scale), width, sinks,
+                  query.data_ptr(), qb, qh, qt, batch, rows, heads, page_heads, dim, pool.group, float(scale), width, sinks,
                   splits, out.data_ptr(), ob, oh, ot, ws.data_ptr(), ws.numel(), _lib.status_ptr(dev), stream)
     return out
 

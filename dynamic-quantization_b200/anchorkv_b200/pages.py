@@ -28,6 +28,9 @@ from .decode import _workspace
 from .pool import PagePool
 
 
+_Slots = ctypes.c_int64 * 6  # first byte and count of the INT4, INT8 and FP16 slots
+
+
 def _check_table(pool: PagePool, table: torch.Tensor, dims) -> None:
     if table.dtype != torch.int64 or table.dim() not in dims or not table.is_cuda:
         raise ValueError("a page table is an int64 CUDA tensor [batch, columns] or [layers, batch, columns]")
@@ -104,11 +107,13 @@ def compact_pages(pool: PagePool, table: torch.Tensor, into: PagePool, live: dic
         raise ValueError("the target pool must have the source's page geometry and device")
     if not into.untouched:
         raise ValueError("the target pool must be a new one: no slot taken, not grown, not shuffled")
-    taken = {b: into.capacity[b] if live is None else int(live.get(b, 0)) for b in (4, 8, 16)}
-    for b, n in taken.items():
-        if n < 0:
-            raise ValueError("page counts must be non-negative")
-        into.check_free(b, n)
+    taken = into.capacity
+    if live is not None:
+        taken = {b: int(live.get(b, 0)) for b in (4, 8, 16)}
+        for b, n in taken.items():
+            if n < 0:
+                raise ValueError("page counts must be non-negative")
+            into.check_free(b, n)
     flat = table.contiguous()
     dev = table.device
     source, target = pool.arena.data_ptr(), into.arena.data_ptr()
@@ -123,7 +128,8 @@ def compact_pages(pool: PagePool, table: torch.Tensor, into: PagePool, live: dic
         status, stream = _lib.status_ptr(dev), _lib.stream_of(dev)
         out = torch.empty_like(flat)
         ws = _workspace(dev, nbytes, stream)
-        slots = (ctypes.c_int64 * 6)(*(v for b in (4, 8, 16) for v in (into.base[b], into.capacity[b])))
+        base, count = into.base, into.capacity
+        slots = _Slots(base[4], count[4], base[8], count[8], base[16], count[16])
         _lib.call("akv_compact_pages", flat.data_ptr(), flat.numel(), out.data_ptr(), pool.arena.data_ptr(),
                   pool.nbytes, into.arena.data_ptr(), into.nbytes, slots, pool.heads, pool.dim, pool.group,
                   ws.data_ptr(), ws.numel(), status, stream)

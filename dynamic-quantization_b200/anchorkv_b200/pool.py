@@ -24,6 +24,8 @@ reference's batch-one ``PagedLayer`` table (packed_decode.py:122-133).
 
 from __future__ import annotations
 
+from functools import cached_property
+
 import numpy as np
 import torch
 
@@ -222,18 +224,22 @@ class PagePool:
 
     def _lay_out(self, heads: int, dim: int, group: int, pages: dict | None) -> None:
         self.heads, self.dim, self.group = heads, dim, group
-        pages = pages or {}
         self.page_bytes = _page_bytes(heads, dim, group)
-        self.base, self.capacity, self._free = {}, {}, {}
+        self.base, self.capacity = {16: 0, 8: 0, 4: 0}, {16: 0, 8: 0, 4: 0}
         cursor = 0
-        for bits in (16, 8, 4):
-            n = int(pages.get(bits, 0))
-            self.base[bits] = cursor
-            self.capacity[bits] = n
-            self._free[bits] = _FreeSlots()
-            self._free[bits].add_run(cursor, self.page_bytes[bits], n)
-            cursor += n * self.page_bytes[bits]
+        if pages:
+            for bits in (16, 8, 4):
+                n = int(pages.get(bits, 0))
+                self.base[bits] = cursor
+                self.capacity[bits] = n
+                self._free[bits].add_run(cursor, self.page_bytes[bits], n)
+                cursor += n * self.page_bytes[bits]
         self.nbytes = max(cursor, 16)
+
+    @cached_property
+    def _free(self) -> dict:
+        """Free slots by precision (made when asked for: a pool that names a caller's memory has none)."""
+        return {bits: _FreeSlots() for bits in (16, 8, 4)}
 
     @classmethod
     def over(cls, arena: torch.Tensor, heads: int, dim: int, *, group: int = 64, pages: dict | None = None) -> "PagePool":

@@ -87,6 +87,38 @@ constexpr int64_t kHeaderBytes = 256;
 // Workspace: the header, then the partial states (kPartialsF holds their
 // offset in 4-byte words).
 
+// Where the output rows lie.  heads_per_kv > 0: a multi-row decode, whose KV
+// head's row r is query token r / heads_per_kv of query head r % heads_per_kv.
+struct OutRows {
+  int64_t bs, hs, ts;
+  int32_t heads_per_kv;
+  // Element offset of row h = kvh * gqa + r of sequence b.
+  __device__ __forceinline__ int64_t at(int b, int h, int kvh, int r) const {
+    if (heads_per_kv == 0) return (int64_t)b * bs + (int64_t)h * hs;
+    const int t = r / heads_per_kv;
+    return (int64_t)b * bs + (int64_t)(kvh * heads_per_kv + (r - t * heads_per_kv)) * hs + (int64_t)t * ts;
+  }
+};
+
+// Write one merged row: the normalised fp16 output (at `out`) and/or the (acc, m, l) state.
+template <int D>
+__device__ __forceinline__ void store_row(int lane, int b, int h, int q_heads, float m, float l,
+                                          const float (&acc)[D / 32], __half *out, float *state) {
+  constexpr int VEC = D / 32, RS = D + 2;
+  if (out) {
+    __half *o = out + VEC * lane;
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) o[i] = __float2half_rn(acc[i] * inv);
+  }
+  if (state) {
+    float *st = state + ((int64_t)b * q_heads + h) * RS;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) st[VEC * lane + i] = acc[i];
+    if (lane == 0) st[D] = m, st[D + 1] = l;
+  }
+}
+
 struct DecodeParams {
   const uint8_t *arena;
   int64_t arena_bytes;
@@ -106,6 +138,9 @@ struct DecodeParams {
   int32_t uniform_tokens, rows, heads_per_kv, columns, window, sinks, lead;
   int64_t q_ts;
   FastDiv fd_hpk;
+  // Not null: a CTA has one whole item, `range` pages a warp, and writes its outputs itself.
+  __half *out;
+  OutRows to;
   float scale_log2;
   int32_t *header;
   float *partials;
@@ -627,9 +662,10 @@ __global__ void __launch_bounds__(DecodeTraits<D>::kMaxThreads, 1)
   const int gw = blockIdx.x * (blockDim.x >> 5) + warp;  // warps per CTA are chosen at launch
   const int mb = p.max_blocks;
   const int total = p.items * mb;
-  const int e_begin = gw * p.range;
-  const int e_end = min(e_begin + p.range, total);
-  if (gw >= p.warps || e_begin >= e_end) return;  // whole warps only; no CTA-wide barriers below
+  const bool own_item = ROWS && p.out != nullptr;
+  const int e_begin = own_item ? (int)blockIdx.x * mb + warp * p.range : gw * p.range;
+  const int e_end = min(e_begin + p.range, own_item ? ((int)blockIdx.x + 1) * mb : total);
+  if (gw >= p.warps || e_begin >= e_end) return;  // whole warps only; own_item: none, each has a page
   const int first_item = e_begin / mb, last_seg = (e_end - 1) / mb - first_item;
   const int ipb = p.kv_heads * p.qgroups;
 
@@ -778,7 +814,8 @@ __global__ void __launch_bounds__(DecodeTraits<D>::kMaxThreads, 1)
     const int qg = (item % ipb) % p.qgroups;
     const int nq = min(8, p.gqa - 8 * qg);
     constexpr int PS = D + 4;  // partial row: acc[D], m, l, 2 pad (16-byte aligned rows)
-    float *base = p.partials + ((int64_t)gw * p.smax + seg) * p.slot_heads * PS;
+    // A CTA with an item of its own keeps its warps' states in their rings.
+    float *base = own_item ? reinterpret_cast<float *>(ring) : p.partials + ((int64_t)gw * p.smax + seg) * p.slot_heads * PS;
     // Scalar stores: the accumulators stay in the MMA's register quads (a
     // float2 pairing of (c0, c2) would fight that allocation on every page).
     const int h0 = 2 * t4, h1 = 2 * t4 + 1;
@@ -904,6 +941,33 @@ __global__ void __launch_bounds__(DecodeTraits<D>::kMaxThreads, 1)
     if (cur_seg >= last_seg) break;
     next_segment();
   }
+  if constexpr (ROWS) {
+    if (!own_item) return;
+    __syncthreads();
+    constexpr int PS = D + 4, VEC = D / 32;
+    const int warps = blockDim.x >> 5, qg = first_item % p.qgroups, b = first_item / ipb;
+    const int kvh = (first_item - b * ipb) / p.qgroups, nq = min(8, p.gqa - 8 * qg);
+    for (int n = warp; n < nq; n += warps) {  // a warp per row, lane w holding warp w's weight
+      auto state = [&](int w) { return reinterpret_cast<const float *>(smem + w * T::kWarpBytes) + n * PS; };
+      const float m = lane < warps ? state(lane)[D] : -INFINITY;
+      float top = m;
+#pragma unroll
+      for (int off = 16; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+      const float weight = m == -INFINITY ? 0.f : ex2(m - top);
+      float l = lane < warps ? state(lane)[D + 1] * weight : 0.f;
+#pragma unroll
+      for (int off = 16; off; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+      float acc[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
+      for (int w = 0; w < warps; ++w) {
+        const float x = __shfl_sync(0xffffffffu, weight, w);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[i] += x == 0.f ? 0.f : x * state(w)[VEC * lane + i];
+      }
+      store_row<D>(lane, b, 0, 0, 0.f, l, acc, p.out + p.to.at(b, 0, kvh, 8 * qg + n), nullptr);
+    }
+  }
 }
 
 // The decomposition a merge reads back from the workspace header (the first
@@ -922,38 +986,6 @@ __device__ __forceinline__ bool merge_geom(const int32_t *header, MergeGeom &g) 
   g.warps = f[kWarpsF], g.smax = f[kSmaxF], g.range = f[kRangeF], g.mb = f[kMaxBlocksF];
   g.kv_heads = f[kKvHeadsF], g.qgroups = f[kQGroupsF], g.gqa = f[kGqaF], g.slot_heads = f[kSlotHeadsF];
   return f[kMagic] == kHeaderMagic && f[kHeadDimF] == D;
-}
-
-// Where the output rows lie.  heads_per_kv > 0: a multi-row decode, whose KV
-// head's row r is query token r / heads_per_kv of query head r % heads_per_kv.
-struct OutRows {
-  int64_t bs, hs, ts;
-  int32_t heads_per_kv;
-  // Element offset of row h = kvh * gqa + r of sequence b.
-  __device__ __forceinline__ int64_t at(int b, int h, int kvh, int r) const {
-    if (heads_per_kv == 0) return (int64_t)b * bs + (int64_t)h * hs;
-    const int t = r / heads_per_kv;
-    return (int64_t)b * bs + (int64_t)(kvh * heads_per_kv + (r - t * heads_per_kv)) * hs + (int64_t)t * ts;
-  }
-};
-
-// Write one merged row: the normalised fp16 output (at `out`) and/or the (acc, m, l) state.
-template <int D>
-__device__ __forceinline__ void store_row(int lane, int b, int h, int q_heads, float m, float l,
-                                          const float (&acc)[D / 32], __half *out, float *state) {
-  constexpr int VEC = D / 32, RS = D + 2;
-  if (out) {
-    __half *o = out + VEC * lane;
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) o[i] = __float2half_rn(acc[i] * inv);
-  }
-  if (state) {
-    float *st = state + ((int64_t)b * q_heads + h) * RS;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) st[VEC * lane + i] = acc[i];
-    if (lane == 0) st[D] = m, st[D + 1] = l;
-  }
 }
 
 // Merge the partial states of the warps that touched each (sequence, query
@@ -1464,6 +1496,9 @@ struct RowsArgs {
   const int32_t *tokens;
   int32_t uniform_tokens, rows, heads_per_kv, columns, window, sinks, lead;
   int64_t q_ts;
+  __half *out;  // where an item has a CTA (own_items), else null
+  OutRows to;
+  int32_t warps;  // of such a CTA
 };
 
 // Validate, plan and launch the decode kernel.
@@ -1489,6 +1524,10 @@ static int decode_launch(const void *arena, int64_t arena_bytes, const int64_t *
     return AKV_ERR_INVALID;
   if (workspace_bytes < pl.bytes) return AKV_ERR_INVALID;
   if (rows && pl.smax > kMaxSegments) return AKV_ERR_UNSUPPORTED;
+  if (rows && rows->out) {  // a CTA per item
+    pl.range = (max_blocks + rows->warps - 1) / rows->warps, pl.wpc = (max_blocks + pl.range - 1) / pl.range;
+    pl.ctas = pl.items, pl.warps = pl.items * pl.wpc, pl.smax = 1;
+  }
   DecodeParams p = {};
   p.arena = (const uint8_t *)arena;
   p.arena_bytes = arena_bytes;
@@ -1520,7 +1559,7 @@ static int decode_launch(const void *arena, int64_t arena_bytes, const int64_t *
   if (rows) {
     p.tokens = rows->tokens, p.uniform_tokens = rows->uniform_tokens, p.rows = rows->rows;
     p.heads_per_kv = rows->heads_per_kv, p.columns = rows->columns, p.window = rows->window;
-    p.sinks = rows->sinks, p.lead = rows->lead, p.q_ts = rows->q_ts;
+    p.sinks = rows->sinks, p.lead = rows->lead, p.q_ts = rows->q_ts, p.out = rows->out, p.to = rows->to;
     p.fd_hpk = fast_div((uint32_t)rows->heads_per_kv);
   }
   const bool slab = group == 16 * head_dim;
@@ -1739,6 +1778,17 @@ static bool use_tiles(const ChunkPlan &c, int batch, int kv_heads) {
   const int64_t pages = (int64_t)batch * kv_heads * c.columns, groups = (c.rows_total / kv_heads + 7) / 8;
   return pages * (groups - 6) > 40000;
 }
+// Warps of a CTA that takes a whole item and writes its outputs, without a merge
+// kernel: as many as let every item have a CTA at once.  0: the items are too many or
+// too long for it.
+constexpr int kOwnPages = 16;  // of a warp
+static int own_items(const ChunkPlan &c, int batch, int kv_heads) {
+  const int64_t items = (int64_t)batch * kv_heads * ((c.rows_total / kv_heads + 7) / 8);
+  int warps = DecodeTraits<128>::kMaxWarps;
+  while (warps > 1 && items * warps > 148 * DecodeTraits<128>::kMaxWarps) warps /= 2;
+  if (items * warps > 148 * DecodeTraits<128>::kMaxWarps) return 0;
+  return c.columns > 0 && c.columns <= kOwnPages * warps ? warps : 0;
+}
 }  // namespace akv
 
 extern "C" int64_t akv_chunk_workspace_bytes(int32_t batch, int32_t rows, int32_t q_heads, int32_t kv_heads,
@@ -1787,11 +1837,14 @@ extern "C" int akv_chunk_attention(const void *arena, int64_t arena_bytes, const
     a.scale = scale, a.status = dev_status, a.stream = s;
     return chunk_tiles_launch(a, workspace, workspace_bytes);
   }
+  const OutRows to{out_batch_stride, out_head_stride, out_token_stride, c.rows.heads_per_kv};
+  c.rows.warps = own_items(c, batch, kv_heads);
+  if (c.rows.warps > 0) c.rows.out = (__half *)out, c.rows.to = to;
   if (int st = decode_launch(arena, arena_bytes, table, table_stride, seq_blocks, c.columns, query, q_batch_stride,
                              q_head_stride, batch, c.rows_total, kv_heads, head_dim, group, scale, splits, workspace,
                              workspace_bytes, dev_status, s, &c.rows))
     return st;
-  const OutRows to{out_batch_stride, out_head_stride, out_token_stride, c.rows.heads_per_kv};
+  if (c.rows.out) return AKV_OK;
   const int32_t *header = (const int32_t *)workspace;
   const cudaError_t err =
       head_dim == 64 ? merge_launch<64>(header, batch, c.rows_total, (__half *)out, to, nullptr, dev_status, s)
