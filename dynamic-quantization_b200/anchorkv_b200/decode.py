@@ -25,14 +25,14 @@ _workspaces: dict = {}
 _workspace_sizes: dict = {}
 
 
-def _workspace_bytes(device: torch.device, *geometry) -> int:
-    """akv_workspace_bytes for ``geometry`` on ``device``, remembered (it depends only on them)."""
-    key = (device.index, geometry)
+def _workspace_bytes(device: torch.device, *geometry, entry: str = "akv_workspace_bytes") -> int:
+    """What ``entry`` says for ``geometry`` on ``device``, remembered (it depends only on them)."""
+    key = (device.index, entry, geometry)
     nbytes = _workspace_sizes.get(key)
     if nbytes is None:
         if len(_workspace_sizes) > 4096:
             _workspace_sizes.clear()
-        nbytes = _lib.load().akv_workspace_bytes(*geometry)
+        nbytes = getattr(_lib.load(), entry)(*geometry)
         _workspace_sizes[key] = nbytes
     return nbytes
 
@@ -40,18 +40,6 @@ def _workspace_bytes(device: torch.device, *geometry) -> int:
 # Pieces a (sequence, KV head, 8 rows) item of a chunk is cut into at least where it
 # has the pages, as packed_attention's default.
 _CHUNK_SPLITS = 4
-
-
-def _chunk_bytes(device: torch.device, *geometry) -> int:
-    """akv_chunk_workspace_bytes for ``geometry`` on ``device``, remembered as _workspace_bytes does."""
-    key = (device.index, "chunk", geometry)
-    nbytes = _workspace_sizes.get(key)
-    if nbytes is None:
-        if len(_workspace_sizes) > 4096:
-            _workspace_sizes.clear()
-        nbytes = _lib.load().akv_chunk_workspace_bytes(*geometry)
-        _workspace_sizes[key] = nbytes
-    return nbytes
 
 
 _MAX_WORKSPACES = 64
@@ -241,7 +229,8 @@ def _by_position(query, layer, scale, splits, window, sinks, out):
     sinks = min(sinks, 1 << 30)
     ob, oh, ot, _ = out.stride()
     with _lib.on_device(dev):
-        nbytes = _chunk_bytes(dev, batch, rows, heads, page_heads, dim, max_blocks, width, sinks, splits)
+        nbytes = _workspace_bytes(dev, batch, rows, heads, page_heads, dim, max_blocks, width, sinks, splits,
+                                  entry="akv_chunk_workspace_bytes")
         if nbytes < 0:
             raise ValueError('unsupported decode geometry')
         stream = _lib.stream_of(dev)

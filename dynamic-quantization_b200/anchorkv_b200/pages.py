@@ -24,7 +24,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .decode import _workspace
+from .decode import _workspace, _workspace_bytes
 from .pool import PagePool
 
 
@@ -122,7 +122,8 @@ def compact_pages(pool: PagePool, table: torch.Tensor, into: PagePool, live: dic
     if flat.numel() == 0:
         return flat.clone()
     with _lib.on_device(dev):
-        nbytes = _lib.load().akv_compact_workspace_bytes(flat.numel(), pool.nbytes, pool.heads, pool.dim, pool.group)
+        nbytes = _workspace_bytes(dev, flat.numel(), pool.nbytes, pool.heads, pool.dim, pool.group,
+                                  entry="akv_compact_workspace_bytes")
         if nbytes < 0:
             raise ValueError("unsupported page geometry")
         status, stream = _lib.status_ptr(dev), _lib.stream_of(dev)

@@ -39,6 +39,15 @@
 //    the caller's workspace; the merge kernel combines the few warps that
 //    share an item.  The workspace starts with a header describing the
 //    decomposition, so merging needs nothing but the workspace.
+//  * windowed decode and chunks run the same loop (ROWS): a KV head's rows are
+//    its (query token, query head) pairs, 8 an item, and an item's pages the
+//    columns its rows can see.  Where items are few or short each gets a CTA
+//    whose warps join their states in shared memory (OWN): 512 tokens through a
+//    window of 128, one sequence, 18.4 us a call against 23.7 with the merge.
+//    Long windows are bound as the plain decode by dequantisation, several rows
+//    a KV head by doing it once per 8 rows: 5 drafted tokens over 8192, 16
+//    sequences, 92 us, 2.5 TB/s of pages (a variant with 16 rows an item needed
+//    more registers than 16 warps an SM leave and was slower).
 #include <math.h>
 
 #include <string.h>
@@ -46,6 +55,7 @@
 #include <algorithm>
 #include <atomic>
 #include <mutex>
+#include <type_traits>
 
 #include "akv_chunk.cuh"
 #include "akv_common.cuh"
@@ -138,7 +148,7 @@ struct DecodeParams {
   int32_t uniform_tokens, rows, heads_per_kv, columns, window, sinks, lead;
   int64_t q_ts;
   FastDiv fd_hpk;
-  // Not null: a CTA has one whole item, `range` pages a warp, and writes its outputs itself.
+  // OWN: where the outputs go; a CTA has one item, `range` pages a warp.
   __half *out;
   OutRows to;
   float scale_log2;
@@ -637,7 +647,10 @@ __device__ __forceinline__ void query_fragments(const uint32_t (&qw)[D / 8], uin
 // share every page a warp streams; an item's entries are the page columns its
 // rows can see (the columns of the first `sinks` tokens, then those from the
 // oldest row's window on), and pages at the borders are masked by position.
-template <int D, bool SLAB, bool ROWS>
+// OWN (of a multi-row decode): a CTA has one whole item, whose pages its warps share
+// out; they join their states in shared memory and write the item's outputs, and no
+// merge kernel follows.  A variant of its own, so that the others keep their registers.
+template <int D, bool SLAB, bool ROWS, bool OWN>
 __global__ void __launch_bounds__(DecodeTraits<D>::kMaxThreads, 1)
     decode_streamk_kernel(const DecodeParams p) {
   using T = DecodeTraits<D>;
@@ -662,11 +675,10 @@ __global__ void __launch_bounds__(DecodeTraits<D>::kMaxThreads, 1)
   const int gw = blockIdx.x * (blockDim.x >> 5) + warp;  // warps per CTA are chosen at launch
   const int mb = p.max_blocks;
   const int total = p.items * mb;
-  const bool own_item = ROWS && p.out != nullptr;
-  const int e_begin = own_item ? (int)blockIdx.x * mb + warp * p.range : gw * p.range;
-  const int e_end = min(e_begin + p.range, own_item ? ((int)blockIdx.x + 1) * mb : total);
-  if (gw >= p.warps || e_begin >= e_end) return;  // whole warps only; own_item: none, each has a page
-  const int first_item = e_begin / mb, last_seg = (e_end - 1) / mb - first_item;
+  const int e_begin = OWN ? (int)blockIdx.x * mb + warp * p.range : gw * p.range;
+  const int e_end = min(e_begin + p.range, OWN ? ((int)blockIdx.x + 1) * mb : total);
+  if (gw >= p.warps || e_begin >= e_end) return;  // whole warps only; OWN: none, each has a page
+  const int first_item = OWN ? (int)blockIdx.x : e_begin / mb, last_seg = OWN ? 0 : (e_end - 1) / mb - first_item;
   const int ipb = p.kv_heads * p.qgroups;
 
   uint8_t *ring = smem + warp * T::kWarpBytes;
@@ -814,8 +826,9 @@ __global__ void __launch_bounds__(DecodeTraits<D>::kMaxThreads, 1)
     const int qg = (item % ipb) % p.qgroups;
     const int nq = min(8, p.gqa - 8 * qg);
     constexpr int PS = D + 4;  // partial row: acc[D], m, l, 2 pad (16-byte aligned rows)
-    // A CTA with an item of its own keeps its warps' states in their rings.
-    float *base = own_item ? reinterpret_cast<float *>(ring) : p.partials + ((int64_t)gw * p.smax + seg) * p.slot_heads * PS;
+    float *base;
+    if constexpr (OWN) base = reinterpret_cast<float *>(ring);  // its records are consumed
+    else base = p.partials + ((int64_t)gw * p.smax + seg) * p.slot_heads * PS;
     // Scalar stores: the accumulators stay in the MMA's register quads (a
     // float2 pairing of (c0, c2) would fight that allocation on every page).
     const int h0 = 2 * t4, h1 = 2 * t4 + 1;
@@ -901,17 +914,19 @@ __global__ void __launch_bounds__(DecodeTraits<D>::kMaxThreads, 1)
     }
     const uint32_t meta = slot_meta[slot];
     uint8_t *rec = ring + slot_phys[slot];
-    const int seg = (int)(meta >> 16);
-    while (cur_seg < seg) {
-      finalize(cur_seg);
-      next_segment();
+    if constexpr (!OWN) {
+      const int seg = (int)(meta >> 16);
+      while (cur_seg < seg) {
+        finalize(cur_seg);
+        next_segment();
+      }
     }
     const int ntok = (int)((meta >> 4) & 31), ntok1 = (int)((meta >> 9) & 31);
     const bool has2 = (meta & 4u) != 0;
     const bool partial = ROWS && (meta & 8u);
     int2 cols = make_int2(0, 0);
     if (partial) cols = slot_cols[slot];
-    const int item = first_item + cur_seg;
+    const int item = OWN ? first_item : first_item + cur_seg;
     switch (meta & 3u) {
       case AKV_MODE_INT4:
         slot_attend<D, AKV_MODE_INT4, SLAB, ROWS>(rec, rb4, has2, ntok, ntok1, lane, lg, si, qf, p.scale_log2, st, o,
@@ -938,11 +953,10 @@ __global__ void __launch_bounds__(DecodeTraits<D>::kMaxThreads, 1)
   // Items past the last record (or with no visible page) still get a partial.
   while (true) {
     finalize(cur_seg);
-    if (cur_seg >= last_seg) break;
+    if (OWN || cur_seg >= last_seg) break;
     next_segment();
   }
-  if constexpr (ROWS) {
-    if (!own_item) return;
+  if constexpr (OWN) {
     __syncthreads();
     constexpr int PS = D + 4, VEC = D / 32;
     const int warps = blockDim.x >> 5, qg = first_item % p.qgroups, b = first_item / ipb;
@@ -1421,8 +1435,9 @@ static int device_ctas(int *out) {
     per_sm = per_sm == 0 ? n : std::min(per_sm, n);
     return true;
   };
-  if (!fit(decode_streamk_kernel<D, false, false>) || !fit(decode_streamk_kernel<D, true, false>) ||
-      !fit(decode_streamk_kernel<D, false, true>) || !fit(decode_streamk_kernel<D, true, true>))
+  if (!fit(decode_streamk_kernel<D, false, false, false>) || !fit(decode_streamk_kernel<D, true, false, false>) ||
+      !fit(decode_streamk_kernel<D, false, true, false>) || !fit(decode_streamk_kernel<D, true, true, false>) ||
+      !fit(decode_streamk_kernel<D, false, true, true>) || !fit(decode_streamk_kernel<D, true, true, true>))
     return AKV_ERR_CUDA;
   if (per_sm < 1) return AKV_ERR_CUDA;
   *out = sms * per_sm;
@@ -1564,16 +1579,22 @@ static int decode_launch(const void *arena, int64_t arena_bytes, const int64_t *
   }
   const bool slab = group == 16 * head_dim;
   cudaError_t err;
-  auto launch = [&](auto wide, auto kernel_slab_rows, auto kernel_rows, auto kernel_slab, auto kernel) {
-    return launch_dependent(rows ? (slab ? kernel_slab_rows : kernel_rows) : (slab ? kernel_slab : kernel), pl.ctas,
-                            pl.wpc * 32, pl.wpc * decltype(wide)::kWarpBytes, s, p);
+  auto launch = [&](auto wide, auto kernel) {
+    return launch_dependent(kernel, pl.ctas, pl.wpc * 32, pl.wpc * decltype(wide)::kWarpBytes, s, p);
   };
-  if (head_dim == 64)
-    err = launch(DecodeTraits<64>{}, decode_streamk_kernel<64, true, true>, decode_streamk_kernel<64, false, true>,
-                 decode_streamk_kernel<64, true, false>, decode_streamk_kernel<64, false, false>);
-  else
-    err = launch(DecodeTraits<128>{}, decode_streamk_kernel<128, true, true>, decode_streamk_kernel<128, false, true>,
-                 decode_streamk_kernel<128, true, false>, decode_streamk_kernel<128, false, false>);
+  auto choose = [&](auto dim) {
+    constexpr int D = decltype(dim)::value;
+    const DecodeTraits<D> wide;
+    if (rows && rows->out)
+      return slab ? launch(wide, decode_streamk_kernel<D, true, true, true>)
+                  : launch(wide, decode_streamk_kernel<D, false, true, true>);
+    if (rows)
+      return slab ? launch(wide, decode_streamk_kernel<D, true, true, false>)
+                  : launch(wide, decode_streamk_kernel<D, false, true, false>);
+    return slab ? launch(wide, decode_streamk_kernel<D, true, false, false>)
+                : launch(wide, decode_streamk_kernel<D, false, false, false>);
+  };
+  err = head_dim == 64 ? choose(std::integral_constant<int, 64>{}) : choose(std::integral_constant<int, 128>{});
   return err == cudaSuccess ? AKV_OK : AKV_ERR_CUDA;
 }
 
@@ -1780,14 +1801,21 @@ static bool use_tiles(const ChunkPlan &c, int batch, int kv_heads) {
 }
 // Warps of a CTA that takes a whole item and writes its outputs, without a merge
 // kernel: as many as let every item have a CTA at once.  0: the items are too many or
-// too long for it.
-constexpr int kOwnPages = 16;  // of a warp
+// too long for it.  Measured on a B200 against equal ranges and a merge (us, cold
+// cache, INT4, 16 heads over 8 of 128; fill: the items' warps over those that fit):
+//   8 pages a warp     fill 0.05: 22.5 against 18.4   0.65: 34.8, 20.5   0.97: 36.9, 22.5
+//   16 pages a warp    fill 0.22: 24.6 against 28.7   0.54: 32.8, 30.7   0.97: 47.1, 32.8
+//   32 pages a warp    fill 0.65: 51.2 against 51.2   0.86: 55.3, 53.2   0.97: 67.6, 53.2
+//   64 pages a warp    fill 0.86: 92.2 against 98.3   0.97: 104.4, 98.3
 static int own_items(const ChunkPlan &c, int batch, int kv_heads) {
+  constexpr int kDevice = 148 * DecodeTraits<128>::kMaxWarps;
   const int64_t items = (int64_t)batch * kv_heads * ((c.rows_total / kv_heads + 7) / 8);
+  if (items > kDevice || c.columns == 0) return 0;
   int warps = DecodeTraits<128>::kMaxWarps;
-  while (warps > 1 && items * warps > 148 * DecodeTraits<128>::kMaxWarps) warps /= 2;
-  if (items * warps > 148 * DecodeTraits<128>::kMaxWarps) return 0;
-  return c.columns > 0 && c.columns <= kOwnPages * warps ? warps : 0;
+  while (items * warps > kDevice) warps /= 2;
+  const double fill = (double)(items * warps) / kDevice;
+  const int pages = fill >= 0.8 ? 32 : (fill >= 0.5 ? 16 : 8);  // of a warp
+  return c.columns <= pages * warps ? warps : 0;
 }
 }  // namespace akv
 

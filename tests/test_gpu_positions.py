@@ -414,3 +414,18 @@ def test_a_store_under_visibility_rules_has_no_positions(cuda):
     with pytest.raises(ValueError, match="token counts"):
         akv.chunk_attention(q, cache, .1)
     _clean(cuda)
+
+
+@pytest.mark.parametrize("dim,hq,hkv,window,sinks", [(128, 16, 8, 30000, 77), (64, 24, 2, 20001, 0),
+                                                     (128, 4, 4, 40000, 5), (64, 8, 8, 9000, 8000)])
+def test_long_windows_of_single_tokens(cuda, dim, hq, hkv, window, sinks):
+    """Items of many pages, cut between warps and joined by the merge."""
+    lengths = [33000, 20007, 5]
+    store, k, v = _fp16_store(cuda, lengths, dim, heads=hkv, seed=window)
+    q = _normal(cuda, 3, (3, hq, 1, dim))
+    out = akv.packed_attention(q, store, dim ** -.5, window=window, sinks=sinks)
+    assert_rows_close(out, *_expected(q, k, v, lengths, dim ** -.5, window, sinks))
+    several = _normal(cuda, 4, (3, hq, 3, dim))
+    out = akv.chunk_attention(several, store, dim ** -.5, window=window, sinks=sinks)
+    assert_rows_close(out, *_expected(several, k, v, lengths, dim ** -.5, window, sinks))
+    _clean(cuda)
