@@ -141,7 +141,7 @@ struct DecodeParams {
   int32_t batch, q_heads, kv_heads, gqa, qgroups, items, log2_group;
   int32_t warps, range, smax, slot_heads;
   FastDiv fd_mb, fd_ipb, fd_qgroups;  // max_blocks, kv_heads * qgroups, qgroups
-  // Multi-row decode (RowsTag): `rows` query tokens per sequence, the last of
+  // Multi-row decode (ROWS): `rows` query tokens per sequence, the last of
   // its `tokens` (or uniform_tokens), gqa counting rows x query heads per KV
   // head; max_blocks is then the columns an item may see (visible_columns).
   const int32_t *tokens;
