@@ -204,7 +204,7 @@ def _by_position(query, layer, scale, splits, window, sinks, out):
     shape, dev = query.shape, query.device
     batch, heads, rows, dim = shape
     if out is None:
-        out = query.new_empty(shape)
+        out = torch.empty_like(query) if query.is_contiguous() else query.new_empty(shape)
     elif out.dtype != torch.float16 or out.shape != shape or out.device != dev or out.stride(-1) != 1:
         raise ValueError("out must be an FP16 tensor of the query's shape on its device, unit stride in head_dim")
     pool = layer.pool

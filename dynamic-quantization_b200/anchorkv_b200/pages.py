@@ -81,7 +81,7 @@ def fork_pages(pool: PagePool, table: torch.Tensor, parents: torch.Tensor, fresh
         three = three.contiguous()
     with _lib.on_device(dev):
         status, stream = _lib.status_ptr(dev), _lib.stream_of(dev)
-        out = torch.empty((layers, children, columns), dtype=torch.int64, device=dev)
+        out = three.new_empty((layers, children, columns))
         if out.numel():
             _lib.call("akv_fork_pages", three.data_ptr(), three.stride(0), three.stride(1), layers, batch, columns,
                       None if counts is None else counts.data_ptr(), uniform, parents.data_ptr(), children,

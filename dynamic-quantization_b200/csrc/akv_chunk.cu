@@ -745,7 +745,8 @@ __global__ void __launch_bounds__(1024) chunk_plan_kernel(const __grid_constant_
   int64_t *list = w.lists + (int64_t)b * w.tiles_max * kTilePages;
   PageList *metas = w.metas + (int64_t)b * w.tiles_max;
   int n = 0;
-  for (int base = 0; base < view.total; base += 1024) {
+  const int threads = blockDim.x, all_warps = threads / 32;
+  for (int base = 0; base < view.total; base += threads) {
     const int v = base + (int)threadIdx.x;
     int64_t d = 0;
     int col = 0;
@@ -763,7 +764,7 @@ __global__ void __launch_bounds__(1024) chunk_plan_kernel(const __grid_constant_
     if (lane == 0) warps[warp] = __popc(mask);
     __syncthreads();
     int before = 0, all = 0;
-    for (int i = 0; i < 32; ++i) {
+    for (int i = 0; i < all_warps; ++i) {
       if (i == warp) before = all;
       all += warps[i];
     }
@@ -797,7 +798,7 @@ __global__ void __launch_bounds__(1024) chunk_plan_kernel(const __grid_constant_
   int4 *ranges = w.ranges + (int64_t)b * p.blocks;
   int *prefix = w.prefix + (int64_t)b * (p.blocks + 1);
   int sum = 0;
-  for (int base = 0; base < p.blocks; base += 1024) {
+  for (int base = 0; base < p.blocks; base += threads) {
     const int m = base + (int)threadIdx.x;
     int cost = 0;
     if (m < p.blocks) {
@@ -818,7 +819,7 @@ __global__ void __launch_bounds__(1024) chunk_plan_kernel(const __grid_constant_
     if (lane == 31) warps[warp] = upto;
     __syncthreads();
     int before = 0, all = 0;
-    for (int i = 0; i < 32; ++i) {
+    for (int i = 0; i < all_warps; ++i) {
       if (i == warp) before = all;
       all += warps[i];
     }
@@ -903,58 +904,72 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_tiles_kernel(const __gr
 }
 
 // ------------------------------------------------------------------- merge
-// Join the partial (O, m, l) rows of the units that the ranges cut, a warp per row; a
-// share that saw nothing (m = -inf) weighs 0.  CTA c's entry of `cuts`: y, z, w - 1 the
-// unit (sequence, KV head, row block) that its range begins and does not end (w 0:
+// Join the partial (O, m, l) rows of the units that the ranges cut, a warp for four
+// rows; a share that saw nothing (m = -inf) weighs 0.  CTA c's entry of `cuts`: y, z, w - 1
+// the unit (sequence, KV head, row block) that its range begins and does not end (w 0:
 // none); x: it goes on with a unit begun before (1), and ends it (2).  Block c joins
 // the unit that range c begins.
+constexpr int kMergeRows = 4;  // of a warp, whose loads are in flight together
 template <int D>
 __global__ void __launch_bounds__(256) chunk_merge_kernel(const __grid_constant__ ChunkParams p) {
-  constexpr int VEC = D / 32, kRowStride = D + 4;
+  constexpr int VEC = D / 32, kRowStride = D + 4, R = kMergeRows, CB = 2;  // CB shares of each row at a time
   grid_dependency_wait();
   allow_dependents_launch();
   const ChunkArgs &a = p.a;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c0 = blockIdx.x;
   const int4 cut = __ldcg(p.w.cuts + c0);
-  const int b = cut.y, kvh = cut.z, row0 = 256 * (cut.w - 1), r = blockIdx.y * 8 + warp;
-  if (cut.w == 0 || r >= p.rows_kv - row0) return;
+  const int b = cut.y, kvh = cut.z, row0 = 256 * (cut.w - 1), r0 = blockIdx.y * 8 * R + warp;
+  const int rows = min(256, p.rows_kv - row0);
+  if (cut.w == 0 || r0 >= rows) return;
   int c1 = c0 + 1;
   while (c1 < p.ctas - 1 && __ldcg(&p.w.cuts[c1].x) == 1) ++c1;
-  float m = -INFINITY, l = 0.f, acc[VEC];
+  float m[R], l[R], acc[R][VEC];
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
-  constexpr int CB = 4;  // shares whose loads are in flight together
+  for (int k = 0; k < R; ++k) {
+    m[k] = -INFINITY, l[k] = 0.f;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) acc[k][i] = 0.f;
+  }
   for (int c = c0; c <= c1; c += CB) {
-    float2 ml[CB];
-    float o[CB][VEC];
+    float2 ml[R][CB];
+    float o[R][CB][VEC];
 #pragma unroll
-    for (int j = 0; j < CB; ++j) {
-      ml[j].x = -INFINITY;
-      if (c + j <= c1) {
-        const float *part = p.partials + ((2ll * (c + j) + (c + j == c0 ? 1 : 0)) * 256 + r) * kRowStride;
-        ml[j] = __ldcg(reinterpret_cast<const float2 *>(part + D));
+    for (int k = 0; k < R; ++k)
 #pragma unroll
-        for (int i = 0; i < VEC; i += 2) {
-          const float2 v = __ldcg(reinterpret_cast<const float2 *>(part + VEC * lane + i));
-          o[j][i] = v.x, o[j][i + 1] = v.y;
+      for (int j = 0; j < CB; ++j) {
+        ml[k][j].x = -INFINITY;
+        if (c + j <= c1 && r0 + 8 * k < rows) {
+          const float *part = p.partials + ((2ll * (c + j) + (c + j == c0 ? 1 : 0)) * 256 + r0 + 8 * k) * kRowStride;
+          ml[k][j] = __ldcg(reinterpret_cast<const float2 *>(part + D));
+#pragma unroll
+          for (int i = 0; i < VEC; i += 2) {
+            const float2 v = __ldcg(reinterpret_cast<const float2 *>(part + VEC * lane + i));
+            o[k][j][i] = v.x, o[k][j][i + 1] = v.y;
+          }
         }
       }
-    }
 #pragma unroll
-    for (int j = 0; j < CB; ++j) {
-      if (ml[j].x == -INFINITY) continue;
-      const float top = fmaxf(m, ml[j].x), x = ex2(m - top), y = ex2(ml[j].x - top);
-      l = l * x + ml[j].y * y;
+    for (int k = 0; k < R; ++k)
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) acc[i] = acc[i] * x + o[j][i] * y;
-      m = isnan(ml[j].x) ? ml[j].x : top;
-    }
+      for (int j = 0; j < CB; ++j) {
+        if (ml[k][j].x == -INFINITY) continue;
+        const float top = fmaxf(m[k], ml[k][j].x), x = ex2(m[k] - top), y = ex2(ml[k][j].x - top);
+        l[k] = l[k] * x + ml[k][j].y * y;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[k][i] = acc[k][i] * x + o[k][j][i] * y;
+        m[k] = isnan(ml[k][j].x) ? ml[k][j].x : top;
+      }
   }
-  const int rho = row0 + r, tok = fdiv(rho, p.fd_hpk), h = kvh * p.heads_per_kv + (rho - tok * p.heads_per_kv);
-  __half *out = a.out + (int64_t)b * a.o_bs + (int64_t)h * a.o_hs + (int64_t)tok * a.o_ts + VEC * lane;
-  const float inv = l > 0.f ? 1.f / l : l;
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) out[i] = __float2half_rn(acc[i] * inv);
+  for (int k = 0; k < R; ++k) {
+    const int r = r0 + 8 * k;
+    if (r >= rows) break;
+    const int rho = row0 + r, tok = fdiv(rho, p.fd_hpk), h = kvh * p.heads_per_kv + (rho - tok * p.heads_per_kv);
+    __half *out = a.out + (int64_t)b * a.o_bs + (int64_t)h * a.o_hs + (int64_t)tok * a.o_ts + VEC * lane;
+    const float inv = l[k] > 0.f ? 1.f / l[k] : l[k];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) out[i] = __float2half_rn(acc[k][i] * inv);
+  }
 }
 
 // ------------------------------------------------------------------- host
@@ -991,7 +1006,9 @@ static cudaError_t launch_tiles(const ChunkParams &p) {
   static std::atomic<bool> ready[256];
   if (cudaError_t err = chunk_ready(chunk_tiles_kernel<D>, smem, kTileRegs, ready)) return err;
   cudaStream_t s = p.a.stream;
-  if (cudaError_t err = launch_dependent(chunk_plan_kernel, p.a.batch, 1024, 0, s, p)) return err;
+  // few columns: fewer warps meet at the barriers of the one step they take
+  const int planners = p.w.tiles_max * kTilePages <= 512 ? 256 : 1024;
+  if (cudaError_t err = launch_dependent(chunk_plan_kernel, p.a.batch, planners, 0, s, p)) return err;
   // 16 KV-head-pages a warp where there are tiles enough for the device, down to one
   const int64_t tiles = (int64_t)p.w.tiles_max * p.a.batch;
   const int jobs = std::min(2 * kTilePages * p.a.kv_heads / 8, 65535);  // of a tile, per warp of a CTA
@@ -1001,7 +1018,7 @@ static cudaError_t launch_tiles(const ChunkParams &p) {
             launch_dependent(chunk_unpack_kernel<D, SLAB>, dim3(p.w.tiles_max, p.a.batch, parts), 256, 0, s, p))
       return err;
   if (cudaError_t err = launch_dependent(chunk_tiles_kernel<D>, p.ctas, kTileThreads, smem, s, p)) return err;
-  return launch_dependent(chunk_merge_kernel<D>, dim3(p.ctas, std::min(32, (p.rows_kv + 7) / 8)), 256, 0, s, p);
+  return launch_dependent(chunk_merge_kernel<D>, dim3(p.ctas, std::min(256, p.rows_kv + 8 * kMergeRows - 1) / (8 * kMergeRows)), 256, 0, s, p);
 }
 
 static int64_t align256(int64_t n) { return (n + 255) & ~(int64_t)255; }
