@@ -101,7 +101,8 @@ def compact_pages(pool: PagePool, table: torch.Tensor, into: PagePool, live: dic
     ``into``: a pool of the same page geometry over another arena, with no slot
     taken and room for the pages.  ``live``: distinct pages of each precision
     (bits -> count), which ``into`` then counts as taken; by default all of its
-    slots.  ``pool`` and ``table`` are left as they are."""
+    slots.  Pages beyond them stay behind: their entries become skip entries and
+    the next call raises KernelError.  ``pool`` and ``table`` are left as they are."""
     _check_table(pool, table, range(1, 9))
     if (into.heads, into.dim, into.group) != (pool.heads, pool.dim, pool.group) or into.arena.device != table.device:
         raise ValueError("the target pool must have the source's page geometry and device")
@@ -129,8 +130,8 @@ def compact_pages(pool: PagePool, table: torch.Tensor, into: PagePool, live: dic
         status, stream = _lib.status_ptr(dev), _lib.stream_of(dev)
         out = torch.empty_like(flat)
         ws = _workspace(dev, nbytes, stream)
-        base, count = into.base, into.capacity
-        slots = _Slots(base[4], count[4], base[8], count[8], base[16], count[16])
+        base = into.base  # no page goes to a slot that is not counted as taken
+        slots = _Slots(base[4], taken[4], base[8], taken[8], base[16], taken[16])
         _lib.call("akv_compact_pages", flat.data_ptr(), flat.numel(), out.data_ptr(), pool.arena.data_ptr(),
                   pool.nbytes, into.arena.data_ptr(), into.nbytes, slots, pool.heads, pool.dim, pool.group,
                   ws.data_ptr(), ws.numel(), status, stream)

@@ -26,7 +26,7 @@
 // there 1300 (head_dim 64) to 1700 clocks (128) later, behind O += P V, while the other
 // row tile is at its exponentials.  A 2048-token chunk of 32768 (32 heads over 8, 128)
 // takes 905 us, 1.1 PFLOP/s; 1000 tokens through a window of
-// 2048 (4 sequences, 24 heads over 8, 64) 154 us, of which the tiles take 115.
+// 2048 (4 sequences, 24 heads over 8, 64) 150 us, of which the tiles take 115.
 // Slower or no faster were: tiles of 64 tokens with S twice; S a tile ahead of P where
 // head_dim 64 leaves TMEM for it (149 to 157 us against 154); a thread per row tile
 // issuing the MMAs (1296 against 905); exponentials of some pairs by a polynomial

@@ -43,10 +43,10 @@
 //    its (query token, query head) pairs, 8 an item, and an item's pages the
 //    columns its rows can see.  Where items are few or short each gets a CTA
 //    whose warps join their states in shared memory (OWN): 512 tokens through a
-//    window of 128, one sequence, 18.4 us a call against 23.7 with the merge.
+//    window of 128, one sequence, 17 us a call against 23.7 with the merge.
 //    Long windows are bound as the plain decode by dequantisation, several rows
 //    a KV head by doing it once per 8 rows: 5 drafted tokens over 8192, 16
-//    sequences, 92 us, 2.5 TB/s of pages (a variant with 16 rows an item needed
+//    sequences, 91 us, 2.5 TB/s of pages (a variant with 16 rows an item needed
 //    more registers than 16 warps an SM leave and was slower).
 #include <math.h>
 

@@ -6,6 +6,7 @@
 // once and written once (a compacted page that several entries share moves
 // once), and the tables are 8 bytes a page beside 16 to 64 KB of payload.
 #include <algorithm>
+#include <atomic>
 
 #include "akv_common.cuh"
 
@@ -108,8 +109,10 @@ __global__ void __launch_bounds__(kCopyThreads) fork_pages_kernel(const ForkPara
 //   rank   an owner's rank is the owners before it; place[key] = its new offset;
 //   move   owners copy their page, every entry is rewritten through place[key].
 constexpr int kRankThreads = 1024;
-// Entries that one CTA plans: 8192 take it about 8 us, the four kernels' launches cost more.
-constexpr int kOnePlan = 8192;
+// Entries and keys that one CTA plans, in shared memory: it takes about 8 us, the launches
+// of the four kernels of a larger plan cost more.  A call for 3700 entries that name 87 MB
+// of pages: 26 us (27 with the owners in global memory), 13 of them the copy's floor.
+constexpr int kOnePlan = 8192, kOnePlanKeys = 48 << 10;
 
 struct CompactParams {
   const int64_t *table;
@@ -217,8 +220,9 @@ __global__ void __launch_bounds__(kRankThreads) compact_plan_kernel(const Compac
   __shared__ int warps[4][32];
   grid_dependency_wait();
   allow_dependents_launch();
-  uint4 *owner = reinterpret_cast<uint4 *>(p.owner);
-  for (int k = threadIdx.x; k < (keys + 3) / 4; k += kRankThreads) owner[k] = make_uint4(~0u, ~0u, ~0u, ~0u);
+  extern __shared__ __align__(16) uint32_t owner[];
+  for (int k = threadIdx.x; k < (keys + 3) / 4; k += kRankThreads)
+    reinterpret_cast<uint4 *>(owner)[k] = make_uint4(~0u, ~0u, ~0u, ~0u);
   __syncthreads();
   constexpr int N = kOnePlan / kRankThreads;  // entries of a thread, their loads in flight together
   int64_t d[N];
@@ -233,7 +237,7 @@ __global__ void __launch_bounds__(kRankThreads) compact_plan_kernel(const Compac
     key[i] = -1;
     if (movable(p, d[i])) {
       key[i] = desc_offset(d[i]) / p.unit;
-      atomicMin(p.owner + key[i], (uint32_t)(i * kRankThreads + threadIdx.x));
+      atomicMin(owner + key[i], (uint32_t)(i * kRankThreads + threadIdx.x));
     } else if (desc_mode(d[i]) != AKV_MODE_SKIP) {
       set_status(p.status, AKV_DEV_BAD_DESCRIPTOR);
     }
@@ -241,7 +245,7 @@ __global__ void __launch_bounds__(kRankThreads) compact_plan_kernel(const Compac
   __syncthreads();
   uint32_t first[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) first[i] = key[i] >= 0 ? __ldcg(p.owner + key[i]) : ~0u;
+  for (int i = 0; i < N; ++i) first[i] = key[i] >= 0 ? owner[key[i]] : ~0u;
   int before[4] = {0, 0, 0, 0};
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -249,7 +253,10 @@ __global__ void __launch_bounds__(kRankThreads) compact_plan_kernel(const Compac
     const int mode = first[i] == (uint32_t)(i * kRankThreads + threadIdx.x) ? desc_mode(d[i]) : 0;
     int all[4];
     const int rank = block_rank(mode, warps, all);
-    if (mode != 0) set_place(p, d[i], before[mode] + rank);
+    if (mode != 0) {
+      p.owner[key[i]] = first[i];
+      set_place(p, d[i], before[mode] + rank);
+    }
 #pragma unroll
     for (int m = 1; m < 4; ++m) before[m] += all[m];
   }
@@ -286,6 +293,17 @@ static int check_page_geometry(int heads, int head_dim, int group) {
 }
 static bool overlap(const void *a, int64_t a_bytes, const void *b, int64_t b_bytes) {
   return (const uint8_t *)a < (const uint8_t *)b + b_bytes && (const uint8_t *)b < (const uint8_t *)a + a_bytes;
+}
+// Raise the small plan's shared-memory limit, once per device.
+static cudaError_t plan_ready() {
+  static std::atomic<bool> ready[256];
+  int dev = 0;
+  if (cudaError_t err = cudaGetDevice(&dev)) return err;
+  if (dev < 256 && ready[dev].load(std::memory_order_acquire)) return cudaSuccess;
+  if (cudaError_t err = cudaFuncSetAttribute(compact_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * kOnePlanKeys))
+    return err;
+  if (dev < 256) ready[dev].store(true, std::memory_order_release);
+  return cudaSuccess;
 }
 static int64_t round16(int64_t n) { return (n + 15) & ~(int64_t)15; }
 
@@ -371,8 +389,9 @@ extern "C" int akv_compact_pages(const int64_t *table, int64_t entries, int64_t 
   p.status = dev_status;
   cudaStream_t s = (cudaStream_t)stream;
   cudaError_t err;
-  if (entries <= kOnePlan && z.keys <= 8 * kOnePlan) {
-    err = launch_dependent(compact_plan_kernel, 1, kRankThreads, 0, s, p, (int)z.keys);
+  if (entries <= kOnePlan && z.keys <= kOnePlanKeys) {
+    if (plan_ready() != cudaSuccess) return AKV_ERR_CUDA;
+    err = launch_dependent(compact_plan_kernel, 1, kRankThreads, (int)round16(4 * z.keys), s, p, (int)z.keys);
   } else {
     if (cudaMemsetAsync(p.owner, 0xff, 4 * z.keys, s) != cudaSuccess) return AKV_ERR_CUDA;
     compact_mark_kernel<<<(unsigned)std::min<int64_t>((entries + 255) / 256, 4 * 148), 256, 0, s>>>(p);

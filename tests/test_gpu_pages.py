@@ -138,3 +138,19 @@ def test_compaction_reports_what_it_cannot_move(cuda):
     size = pool.page_bytes[16]
     assert got.tolist() == [[P.encode(16, 16, 0), 0, P.encode(16, 16, size)], [0, P.encode(16, 16, 0), 0]]
     assert akv.take_device_status(cuda) == _lib.DEV_BAD_DESCRIPTOR
+
+
+def test_compaction_keeps_to_the_counted_slots(cuda):
+    """More pages than the caller counted: the rest stay behind, and no free slot of the target is written."""
+    pool = _pool(cuda, 2, 128, 64, {16: 4, 4: 3}, 3)
+    pages = [P.encode(16, 16, int(o)) for o in pool.alloc_many(16, 4)] + [P.encode(4, 7, int(o)) for o in pool.alloc_many(4, 3)]
+    for entries in (len(pages), 9000):  # one CTA's plan, and the plan of many
+        table = torch.tensor((pages * (entries // len(pages) + 1))[:entries], device=cuda)
+        into = P.PagePool(2, 128, group=64, pages={16: 6, 4: 6}, device=cuda)
+        got = akv.compact_pages(pool, table, into, {16: 2, 4: 1}).cpu().tolist()
+        size = pool.page_bytes
+        want = [P.encode(16, 16, 0), P.encode(16, 16, size[16]), 0, 0, P.encode(4, 7, into.base[4]), 0, 0]
+        assert got == (want * (entries // len(want) + 1))[:entries]
+        assert akv.take_device_status(cuda) == _lib.DEV_BAD_DESCRIPTOR
+        assert not into.arena[2 * size[16]:into.base[4]].any() and not into.arena[into.base[4] + size[4]:].any()
+        assert [into.free_slots(b) for b in (16, 8, 4)] == [4, 0, 5]
