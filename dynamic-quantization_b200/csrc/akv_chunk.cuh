@@ -26,7 +26,7 @@ struct ChunkArgs {
   cudaStream_t stream;
 };
 
-// Bytes of workspace the call needs (0: none).
+// Bytes of workspace the call needs (-1: unsupported, or no device).
 int64_t chunk_tiles_bytes(const ChunkArgs &a);
 int chunk_tiles_launch(const ChunkArgs &a, void *workspace, int64_t workspace_bytes);
 
