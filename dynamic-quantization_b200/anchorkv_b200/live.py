@@ -414,6 +414,15 @@ def batched_live_cache(source, *, max_tokens: int, group: int = 64, archive_bits
     return _CACHE_CLASS(store)
 
 
+def _route_mask(q_length: int, attention_mask=None, **_) -> None:
+    """The route's mask function (the model library calls it once per kind of layer
+    and forward): there is no mask to make.  Only here does a padding mask
+    ``[batch, tokens]`` show itself; several rows whose padding would be attended are refused."""
+    if q_length > 1 and attention_mask is not None and not bool(attention_mask.all()):
+        raise ValueError("the paged route attends every stored token up to a row's own: a padding mask with hidden "
+                         "tokens cannot be honoured for several query tokens")
+
+
 @contextmanager
 def paged_route(model, cache, backend: str = "packed"):
     """Route ``model``'s attention over ``cache``'s pages for the duration of the
@@ -423,17 +432,27 @@ def paged_route(model, cache, backend: str = "packed"):
     backends, colab_experiment.py:123-148).  The step's keys and values are in the
     pages by then, so tokens that left the recent window within the step are
     attended at the archive precision.  A layer with a ``sliding_window`` attends
-    that many last positions.  On exit
-    the model's attention implementation is restored and the registry entry
-    points back at SDPA, so it keeps no reference to the cache."""
+    that many last positions.
+
+    Rows are causal over every stored token, padding included, and take no other
+    mask: a step of several tokens with an explicit mask (``[batch, heads, rows,
+    tokens]``) or with a padding mask that hides a token raises ValueError.  A step
+    of one token ignores its mask.
+
+    On exit the model's attention implementation is restored and the registry entries
+    point back at SDPA, so they keep no reference to the cache."""
+    from transformers.masking_utils import ALL_MASK_ATTENTION_FUNCTIONS
     from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
 
     if backend not in ("packed", "dense"):
         raise ValueError("backend must be 'packed' or 'dense'")
-    sdpa = ALL_ATTENTION_FUNCTIONS["sdpa"]
+    sdpa, sdpa_mask = ALL_ATTENTION_FUNCTIONS["sdpa"], ALL_MASK_ATTENTION_FUNCTIONS["sdpa"]
     store = cache.store
 
     def attention(module, query, key, value, attention_mask, scaling, **kwargs):
+        if query.shape[2] > 1 and attention_mask is not None:
+            raise ValueError("the paged route's rows are causal: an explicit attention mask cannot be honoured for "
+                             "several query tokens")
         view = store.batch_view(module.layer_idx)
         window = kwargs.get("sliding_window")
         if backend == "dense":
@@ -455,12 +474,14 @@ def paged_route(model, cache, backend: str = "packed"):
 
     previous = model.config._attn_implementation
     ALL_ATTENTION_FUNCTIONS.register(ROUTE, attention)
+    ALL_MASK_ATTENTION_FUNCTIONS.register(ROUTE, _route_mask)
     model.config._attn_implementation = ROUTE
     try:
         yield
     finally:
         model.config._attn_implementation = previous
         ALL_ATTENTION_FUNCTIONS.register(ROUTE, sdpa)
+        ALL_MASK_ATTENTION_FUNCTIONS.register(ROUTE, sdpa_mask)
 
 
 def decode_step(model, cache, tokens: torch.Tensor):
