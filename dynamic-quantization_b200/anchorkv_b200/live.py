@@ -20,7 +20,9 @@ table per layer that :func:`packed_attention` reads as a ``PagedBatch``:
   counts on the device; a fresh page's descriptors reach the table through
   the same launch (one pinned, non-blocking copy of ``batch`` descriptors);
 * when a page leaves the recent window it is demoted for all sequences at
-  once (``akv_repack_pages``) and its FP16 slots return to the pool;
+  once (``akv_repack_pages``) and its FP16 slots return to the pool; pages of a
+  step of several tokens stay FP16 until the step after it, so that its rows
+  attend them as written and rejected drafts can be cropped away;
 * sequences may share pages: ``fork`` gives every new sequence its parent's
   page tables in one ``akv_fork_pages`` launch over all layers and copies only
   half-filled last pages (beam search, several samples of one prompt), ``crop``
@@ -131,8 +133,14 @@ class PagedKVStore:
         self.lengths[layer] = tokens
         self._archived[layer] = max(eligible - 1, -1)
 
-    def append(self, layer: int, key: torch.Tensor, value: torch.Tensor) -> None:
-        """Append ``[batch, heads, rows, dim]`` decode-step K/V to every sequence."""
+    def append(self, layer: int, key: torch.Tensor, value: torch.Tensor, *, archive: bool = True) -> None:
+        """Append ``[batch, heads, rows, dim]`` decode-step K/V to every sequence.
+
+        Pages that leave the recent window are demoted within the call.  With
+        ``archive=False`` only those that earlier steps pushed out of it are; the
+        pages that this step completes or pushes out keep FP16 until the layer's
+        next append, so that the step's rows attend them as they were written and
+        ``crop`` can take the step back.  FP16 slots grow to hold the step."""
         if key.shape != value.shape or key.shape[0] != self.batch or key.shape[1] != self.heads \
                 or key.shape[-1] != self.dim:
             raise ValueError("key/value geometry does not match the store")
@@ -141,6 +149,9 @@ class PagedKVStore:
             raise ValueError("cache geometry or capacity exceeded")
         key, value = P.as_fp16_rows(key), P.as_fp16_rows(value)
         status, stream = _lib.status_ptr(self.device), _lib.stream_of(self.device)
+        if not archive:
+            self._archive(layer)
+            self.pool.reserve(16, self.batch * (-(-(self.lengths[layer] + rows) // P.BLOCK) - self.pages(layer)))
         done = 0
         while done < rows:
             page, row = divmod(self.lengths[layer], P.BLOCK)
@@ -163,7 +174,8 @@ class PagedKVStore:
                       self.heads, self.dim, status, stream)
             self.lengths[layer] += take
             done += take
-            self._archive(layer)
+            if archive:
+                self._archive(layer)
 
     def _archive(self, layer: int) -> None:
         last = self.lengths[layer] // P.BLOCK - self.recent_pages - 1
@@ -384,7 +396,7 @@ def batched_live_cache(source, *, max_tokens: int, group: int = 64, archive_bits
                 return self.store.lengths[layer_idx]
 
             def update(self, key_states, value_states, layer_idx, cache_kwargs=None):
-                self.store.append(layer_idx, key_states, value_states)
+                self.store.append(layer_idx, key_states, value_states, archive=key_states.shape[2] == 1)
                 return key_states, value_states
 
             # the model library's names for what the store does (beam search, samples, drafts)
@@ -430,8 +442,9 @@ def paged_route(model, cache, backend: str = "packed"):
     :func:`packed_attention` and several with :func:`chunk_attention`,
     ``"dense"`` dequantises the pages and runs SDPA (the reference route's two
     backends, colab_experiment.py:123-148).  The step's keys and values are in the
-    pages by then, so tokens that left the recent window within the step are
-    attended at the archive precision.  A layer with a ``sliding_window`` attends
+    pages by then: those of several tokens in FP16, with the pages that were recent
+    before the step; a single token that completes a page demotes the page that
+    leaves the recent window first.  A layer with a ``sliding_window`` attends
     that many last positions.
 
     Rows are causal over every stored token, padding included, and take no other

@@ -4,10 +4,13 @@ masks they take, what precision their rows see and what can be taken back.
 The host tests drive a small model or the store with the kernel calls recorded
 instead of launched; the GPU tests compare whole steps."""
 
+import numpy as np
 import pytest
 import torch
 
-from anchorkv_b200 import live
+import anchorkv_b200 as akv
+from anchorkv_b200 import _lib, live
+from anchorkv_b200 import pool as P
 
 
 class _Reached(Exception):
@@ -81,3 +84,104 @@ def test_the_mask_registry_is_restored():
     with live.paged_route(model, cache):
         assert ALL_MASK_ATTENTION_FUNCTIONS[live.ROUTE] is live._route_mask
     assert ALL_MASK_ATTENTION_FUNCTIONS[live.ROUTE] is ALL_MASK_ATTENTION_FUNCTIONS["sdpa"]
+
+
+HEADS, DIM, LAYERS = 2, 64, 2
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """Record C-ABI calls instead of launching them; keep descriptor arrays on the host."""
+    calls = []
+    monkeypatch.setattr(_lib, "call", lambda name, *args: calls.append(name))
+    monkeypatch.setattr(_lib, "require_cuda", lambda *a, **k: None)
+    monkeypatch.setattr(_lib, "raise_pending", lambda device: None)
+    monkeypatch.setattr(_lib, "status_ptr", lambda device: 0)
+    monkeypatch.setattr(_lib, "stream_of", lambda device: 0)
+    monkeypatch.setattr(P, "to_device", lambda array, device: torch.from_numpy(np.ascontiguousarray(array, np.int64)))
+    return calls
+
+
+def _host_cache(prefix, batch=2, **kw):
+    kv = torch.zeros((batch, HEADS, prefix, DIM), dtype=torch.float16)
+    return live.batched_live_cache([(kv, kv)] * LAYERS, max_tokens=400, device="cpu", **kw)
+
+
+def _step(cache, rows):
+    kv = torch.zeros((cache.store.batch, HEADS, rows, DIM), dtype=torch.float16)
+    for layer in range(LAYERS):
+        cache.update(kv, kv, layer)
+
+
+def _bits(store):
+    assert (store.bits(0) == store.bits(1)).all() and (store.bits(0) == store.bits(0)[:1]).all()
+    named = {b: int((store.bits(0) == b).sum()) * LAYERS for b in (4, 8, 16)}
+    for b in (4, 8, 16):  # no page is shared here: every slot is free or named once
+        assert store.pool.free_slots(b) + named[b] == store.pool.capacity[b]
+    return store.bits(0)[0].tolist()
+
+
+def test_a_step_of_several_tokens_keeps_its_pages_until_the_next(launches):
+    """Pages that were recent before the step, and those that it writes, are FP16 while its rows attend them."""
+    cache = _host_cache(70, recent_pages=2, protected=(1,))
+    assert _bits(cache.store) == [4, 16, 16, 16, 16]              # complete: 4; recent: 2, 3
+    _step(cache, 60)                                              # 130 tokens
+    assert _bits(cache.store) == [4] + [16] * 8
+    _step(cache, 3)                                               # 8 complete pages: 6 and 7 were recent
+    assert _bits(cache.store) == [4, 16, 4, 4, 4, 4] + [16] * 3
+    _step(cache, 1)
+    assert _bits(cache.store) == [4, 16, 4, 4, 4, 4] + [16] * 3
+    _step(cache, 200)                                             # 334 tokens
+    _step(cache, 1)                                               # a single token demotes at once: 20 complete
+    assert _bits(cache.store) == [4, 16] + [4] * 16 + [16] * 3
+    assert cache.store.demotions == 2 * LAYERS * 17
+
+
+@pytest.mark.parametrize("recent", [0, 1])
+def test_rejected_drafts_are_cropped_across_page_borders(launches, recent):
+    cache = _host_cache(30, recent_pages=recent)
+    for keep in (31, 30, 33):
+        _step(cache, 21 if recent else 5)  # completes the page that holds the accepted prefix, and more
+        cache.crop(keep)
+        assert cache.get_seq_length() == keep
+        if keep > 30:
+            cache.crop(30)
+    assert _bits(cache.store) == [16 if recent else 4, 16]
+    _step(cache, 3)
+    _step(cache, 1)                        # accepted: 34 tokens
+    assert _bits(cache.store) == ([4, 16, 16] if recent else [4, 4, 16])
+
+
+def test_an_append_archives_at_once_unless_told(launches):
+    cache = _host_cache(30, recent_pages=0)
+    kv = torch.zeros((2, HEADS, 40, DIM), dtype=torch.float16)
+    for layer in range(LAYERS):
+        cache.store.append(layer, kv, kv)
+    assert _bits(cache.store) == [4, 4, 4, 4, 16]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [2, 37, 150])
+@pytest.mark.parametrize("backend", ["packed", "dense"])
+def test_a_steps_logits_do_not_see_its_own_archive(cuda, backend, rows):
+    """A chunk over an INT4 store against the same chunk over a store whose pages from the recent window on
+    are protected (always FP16): the same pages by value, so the same logits."""
+    from transformers import DynamicCache, Qwen3Config, Qwen3ForCausalLM
+
+    torch.manual_seed(5)
+    config = Qwen3Config(vocab_size=256, hidden_size=256, intermediate_size=256, num_hidden_layers=2,
+                         num_attention_heads=4, num_key_value_heads=2, head_dim=64, attn_implementation="sdpa")
+    model = Qwen3ForCausalLM(config).to(device=cuda, dtype=torch.float16).eval()
+    ids = torch.randint(0, 256, (2, 80 + rows), generator=torch.Generator().manual_seed(6)).to(cuda)
+    logits = []
+    with torch.inference_mode():
+        stock = DynamicCache()
+        model(input_ids=ids[:, :80], past_key_values=stock, use_cache=True, logits_to_keep=1)
+        source = [(layer.keys, layer.values) for layer in stock.layers]
+        for protected in ((), range(4, 20)):  # 5 complete pages, the last one recent
+            cache = live.batched_live_cache(source, max_tokens=300, recent_pages=1, protected=protected, device=cuda)
+            assert cache.store.bits(0)[0].tolist() == [4, 4, 4, 4, 16]
+            with live.paged_route(model, cache, backend):
+                logits.append(live.decode_step(model, cache, ids[:, 80:]))
+    assert torch.equal(logits[0], logits[1])
+    assert akv.take_device_status(cuda) == 0
