@@ -110,14 +110,15 @@ struct OutRows {
   }
 };
 
-// Write one merged row: the normalised fp16 output (at `out`) and/or the (acc, m, l) state.
+// Write one merged row: the normalised fp16 output (at `out`) and/or the (acc, m, l)
+// state.  A row that saw nothing (l 0) is 0, a NaN stays one.
 template <int D>
 __device__ __forceinline__ void store_row(int lane, int b, int h, int q_heads, float m, float l,
                                           const float (&acc)[D / 32], __half *out, float *state) {
   constexpr int VEC = D / 32, RS = D + 2;
   if (out) {
     __half *o = out + VEC * lane;
-    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const float inv = l > 0.f ? 1.f / l : l;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) o[i] = __float2half_rn(acc[i] * inv);
   }
@@ -822,6 +823,10 @@ __global__ void __launch_bounds__(DecodeTraits<D>::kMaxThreads, 1)
       l0 += __shfl_xor_sync(0xffffffffu, l0, off);
       l1 += __shfl_xor_sync(0xffffffffu, l1, off);
     }
+    if constexpr (ROWS) {  // scores that are all NaN leave the max at -inf, a share without weight: it is NaN too
+      if (isnan(l0)) st.m0 = l0;
+      if (isnan(l1)) st.m1 = l1;
+    }
     const int item = first_item + seg;
     const int qg = (item % ipb) % p.qgroups;
     const int nq = min(8, p.gqa - 8 * qg);
@@ -1190,7 +1195,7 @@ __global__ void __launch_bounds__(1024) merge_wide_kernel(const int32_t *__restr
     for (int i = 1; i < VEC; ++i)
       if (lane == i) v = num[i];
     if (out)
-      out[rows.at(b, h, kvh, r) + VEC * warp + lane] = __float2half_rn(v * (den > 0.f ? 1.f / den : 0.f));
+      out[rows.at(b, h, kvh, r) + VEC * warp + lane] = __float2half_rn(v * (den > 0.f ? 1.f / den : den));
     if (state) {
       float *st = state + ((int64_t)b * q_heads + h) * (D + 2);
       st[VEC * warp + lane] = v;
