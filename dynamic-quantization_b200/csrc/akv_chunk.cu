@@ -9,8 +9,11 @@
 //   O = O + P V        tcgen05.mma, P (fp16) in TMEM over S's columns, O in TMEM
 //
 // P is rounded to fp16 because the MMA takes both operands in one 16-bit type and
-// V's values are fp16; m moves only when a tile exceeds it by 2^8 (then O is
-// rescaled), so P <= 2^8 and its rounding is relative, 2^-11 a term.
+// V's values are fp16.  m is the max less 7 when it moves, and moves only when a tile
+// exceeds it by 15 (then O is rescaled), so P <= 2^15 and the row's largest is at least
+// 2^7: a weight is off by 2^-11 of itself down to 2^-21 of the largest, by 2^-32 of the
+// largest below that (with m at the max by 2^-25: small weights behind one large one
+// would be lost, 2^-7 of it over 262144 tokens).
 //
 // A page would be dequantised once per pair of row tiles; chunk_unpack_kernel does it
 // once per call instead, into operand tiles in the workspace, and the attention
@@ -540,7 +543,7 @@ __device__ __forceinline__ void chunk_softmax(const TileWork &work, ChunkShared<
                                               int lane) {
   using Shared = ChunkShared<D>;
   constexpr int kRowStride = D + 4, kOut = D / 2;
-  constexpr float kNegInf = -INFINITY, kSlack = 8.f;
+  constexpr float kNegInf = -INFINITY, kSlack = 15.f, kLift = 7.f;
   const ChunkParams &p = work.p;
   const ChunkArgs &a = p.a;
   const int quarter = warp & 3, half = warp >> 2;
@@ -612,7 +615,7 @@ __device__ __forceinline__ void chunk_softmax(const TileWork &work, ChunkShared<
         // S of this tile came after O of the row tile's tile before it, so O is at rest
         // here.  A NaN score makes the row's max, and with it the row, NaN.
         if (__any_sync(0xffffffffu, !(top <= m + kSlack))) {
-          const float n = max3(m, top, top);
+          const float low = top - kLift, n = max3(m, low, low);
           const float w = n == kNegInf ? 1.f : ex2(m - n);
           l *= w, m = n;
           if (!first) {

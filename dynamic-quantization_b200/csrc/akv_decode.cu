@@ -388,12 +388,15 @@ struct RowView {
 // pages need no reduction).  With NP = 2 the second page is skipped when `two`
 // is false.
 // ROWS: bit 4 r + i of `hide` hides score i of page r from its row; `ntok` is not looked at.
+// The max is kept 7 lower: P <= 2^15, and fp16 holds weights down to 2^-21 of the row's
+// largest with all its bits and loses none above 2^-32 of it, where many small weights
+// behind one large one add up in a long sequence.  (Without ROWS they round to 2^-25 of it.)
 template <int D, int NP, bool ROWS>
 __device__ __forceinline__ void pages_softmax(float (&s)[NP][4], const int (&ntok)[NP], bool two,
                                               int gid, float scale_log2, SoftmaxState &st,
                                               float (&o)[D / 16][4], uint32_t (&b)[NP][2],
                                               bool partial, uint32_t hide) {
-  constexpr float slack = 8.f;
+  constexpr float lift = ROWS ? 7.f : 0.f, slack = 8.f + lift;
   constexpr float kNegInf = -INFINITY;
   float x[NP][4];
   float mx0 = kNegInf, mx1 = kNegInf;
@@ -421,7 +424,7 @@ __device__ __forceinline__ void pages_softmax(float (&s)[NP][4], const int (&nto
       mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, off));
       mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, off));
     }
-    const float n0 = fmaxf(st.m0, mx0), n1 = fmaxf(st.m1, mx1);
+    const float n0 = fmaxf(st.m0, mx0 - lift), n1 = fmaxf(st.m1, mx1 - lift);
     float a0 = ex2(st.m0 - n0), a1 = ex2(st.m1 - n1);
     if constexpr (ROWS) {  // a row that has seen nothing yet has both maxima at -inf
       if (n0 == kNegInf) a0 = 1.f;
