@@ -498,11 +498,11 @@ def paged_route(model, cache, backend: str = "packed"):
 
 
 def decode_step(model, cache, tokens: torch.Tensor):
-    """One batched step.  ``tokens`` ``[batch]`` or ``[batch, 1]`` (a decoded token
-    per sequence) gives last-position logits ``[batch, vocab]``; ``[batch, n]`` (a
+    """One batched step.  ``tokens`` ``[batch]`` (a decoded token per sequence, in any
+    shape of as many elements) gives last-position logits ``[batch, vocab]``; ``[batch, n]`` (a
     prompt's next chunk, or drafted tokens to verify) logits ``[batch, n, vocab]``."""
     position = cache.get_seq_length()
-    rows = tokens.shape[1] if tokens.dim() == 2 else 1
+    rows = tokens.shape[1] if tokens.dim() == 2 and tokens.numel() != cache.store.batch else 1
     out = model(input_ids=tokens.reshape(-1, rows), past_key_values=cache,
                 cache_position=torch.arange(position, position + rows, device=tokens.device),
                 attention_mask={"full_attention": None, "sliding_attention": None}, use_cache=True,

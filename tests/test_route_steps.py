@@ -185,3 +185,20 @@ def test_a_steps_logits_do_not_see_its_own_archive(cuda, backend, rows):
                 logits.append(live.decode_step(model, cache, ids[:, 80:]))
     assert torch.equal(logits[0], logits[1])
     assert akv.take_device_status(cuda) == 0
+
+
+@pytest.mark.parametrize("shape,rows", [((3,), 1), ((3, 1), 1), ((1, 3), 1), ((3, 2), 2), ((3, 3), 3)])
+def test_a_token_per_sequence_comes_in_any_shape(launches, shape, rows):
+    """As many tokens as sequences are one each, as before steps took several."""
+    cache = _host_cache(20, batch=3)
+    given = {}
+
+    def model(input_ids, cache_position, logits_to_keep, **kw):
+        given.update(ids=input_ids, at=cache_position, keep=logits_to_keep)
+        return type("Out", (), {"logits": torch.zeros((*input_ids.shape, 5))})()
+
+    tokens = torch.arange(3 * rows).view(shape)
+    out = live.decode_step(model, cache, tokens)
+    assert given["ids"].tolist() == tokens.reshape(3, rows).tolist()
+    assert given["at"].tolist() == list(range(20, 20 + rows)) and given["keep"] == rows
+    assert out.shape == ((3, 5) if rows == 1 else (3, rows, 5))
