@@ -759,7 +759,7 @@ __global__ void __launch_bounds__(1024) chunk_plan_kernel(const __grid_constant_
     }
     const int mode = desc_mode(d);
     bool ok = mode != AKV_MODE_SKIP;
-    if (ok && !page_in_arena(d, a.kv_heads * record_bytes(a.head_dim, 1 << a.log2_group, mode), a.arena_bytes)) {
+    if (ok && !page_in_arena(d, a.page_heads * record_bytes(a.head_dim, 1 << a.log2_group, mode), a.arena_bytes)) {
       set_status(a.status, AKV_DEV_BAD_DESCRIPTOR);
       ok = false;
     }
@@ -853,7 +853,7 @@ __global__ void __launch_bounds__(256) chunk_unpack_kernel(const __grid_constant
     const int mode = desc_mode(d), ntok = desc_ntok(d);
     const int pos0 = kBlock * __ldcg(&w.metas[(int64_t)b * w.tiles_max + tile].col[i]);
     uint8_t *out = w.tiles + ((((int64_t)b * a.kv_heads + kvh) * w.tiles_max + tile) * 2 + kv) * kOperand;
-    const uint8_t *rec = a.arena + desc_offset(d) + kvh * record_bytes(D, 1 << a.log2_group, mode);
+    const uint8_t *rec = a.arena + desc_offset(d) + (a.kv_first + kvh) * record_bytes(D, 1 << a.log2_group, mode);
     const int64_t pb = payload_bytes(D, mode);
     const __half *sc = reinterpret_cast<const __half *>(rec + 2 * pb) + (kv ? (kBlock * D) >> a.log2_group : 0);
     uint4 raw[NC];
@@ -1054,25 +1054,37 @@ static int64_t chunk_layout(const ChunkArgs &a, int sms, uint8_t *base, ChunkPar
   return at;
 }
 
-// Operand tiles are four times the bytes of INT4 pages and more, so a large batch goes
-// in slices of whole sequences that share a workspace of about this size.
+// Operand tiles are four times the bytes of INT4 pages and more, so a large call goes
+// in slices that share a workspace of at most about this size (unless one KV head of one
+// sequence needs more): slices of whole sequences, or of a sequence's KV heads where
+// even one sequence is too large.
 constexpr int64_t kSpaceBytes = 2ll << 30;
-static ChunkArgs slice_of(ChunkArgs a, int first, int count) {
+static ChunkArgs sized(ChunkArgs a, int batch, int kv_heads) {
+  a.q_heads = a.q_heads / a.kv_heads * kv_heads, a.kv_heads = kv_heads, a.batch = batch;
+  return a;
+}
+static ChunkArgs slice_of(const ChunkArgs &all, int first, int count, int kv_first, int kv_heads) {
+  ChunkArgs a = sized(all, count, kv_heads);
+  const int64_t head = (int64_t)kv_first * (all.q_heads / all.kv_heads);
   a.table += first * a.table_stride;
   if (a.seq_blocks) a.seq_blocks += first;
   if (a.tokens) a.tokens += first;
-  a.q += first * a.q_bs, a.out += first * a.o_bs;
-  a.batch = count;
+  a.q += first * a.q_bs + head * a.q_hs, a.out += first * a.o_bs + head * a.o_hs;
+  a.kv_first = kv_first, a.page_heads = all.kv_heads;
   return a;
 }
-static int slice_batch(const ChunkArgs &a, int sms) {
-  ChunkArgs some = a;
-  some.batch = 1;
-  const int64_t one = chunk_layout(some, sms, nullptr, nullptr);
-  some.batch = 2;
-  const int64_t each = std::max<int64_t>(1, chunk_layout(some, sms, nullptr, nullptr) - one);  // the rest is shared
-  const int64_t fit = 1 + std::max<int64_t>(0, kSpaceBytes - one) / each;
-  return (int)std::min<int64_t>({fit, a.batch, 65535});  // a grid's second dimension
+struct Slice {
+  int batch, kv_heads;
+};
+static Slice slice_size(const ChunkArgs &a, int sms) {
+  auto bytes = [&](int batch, int kv_heads) { return chunk_layout(sized(a, batch, kv_heads), sms, nullptr, nullptr); };
+  auto fit = [](int64_t one, int64_t two) {  // how many, the first of them `one` with what they share
+    return 1 + std::max<int64_t>(0, kSpaceBytes - one) / std::max<int64_t>(1, two - one);
+  };
+  if (bytes(1, a.kv_heads) > kSpaceBytes && a.kv_heads > 1)
+    return Slice{1, (int)std::min<int64_t>(a.kv_heads, fit(bytes(1, 1), bytes(1, 2)))};
+  const int64_t sequences = fit(bytes(1, a.kv_heads), bytes(2, a.kv_heads));
+  return Slice{(int)std::min<int64_t>({sequences, a.batch, 65535}), a.kv_heads};  // a grid's second dimension
 }
 
 // Tiles of a KV head's row blocks are counted in 32 bits.
@@ -1084,9 +1096,8 @@ static bool countable(const ChunkArgs &a) {
 int64_t chunk_tiles_bytes(const ChunkArgs &a) {
   const int sms = device_sms();
   if (sms <= 0 || !countable(a)) return -1;
-  ChunkArgs part = a;
-  part.batch = slice_batch(a, sms);
-  return chunk_layout(part, sms, nullptr, nullptr);
+  const Slice slice = slice_size(a, sms);
+  return chunk_layout(sized(a, slice.batch, slice.kv_heads), sms, nullptr, nullptr);
 }
 
 int chunk_tiles_launch(const ChunkArgs &all, void *workspace, int64_t workspace_bytes) {
@@ -1094,9 +1105,8 @@ int chunk_tiles_launch(const ChunkArgs &all, void *workspace, int64_t workspace_
   if (sms <= 0) return AKV_ERR_CUDA;
   if (!countable(all)) return AKV_ERR_UNSUPPORTED;
   if (workspace_bytes < chunk_tiles_bytes(all)) return AKV_ERR_INVALID;
-  const int step = slice_batch(all, sms);
-  for (int first = 0; first < all.batch; first += step) {
-    const ChunkArgs a = slice_of(all, first, std::min(step, all.batch - first));
+  const Slice slice = slice_size(all, sms);
+  auto launch = [&](const ChunkArgs &a) {
     ChunkParams p = {};
     p.a = a;
     p.heads_per_kv = a.q_heads / a.kv_heads;
@@ -1109,11 +1119,14 @@ int chunk_tiles_launch(const ChunkArgs &all, void *workspace, int64_t workspace_
     p.vector_out = ((uintptr_t)a.out & 15) == 0 && a.o_bs % 8 == 0 && a.o_hs % 8 == 0 && a.o_ts % 8 == 0;
     chunk_layout(a, sms, (uint8_t *)workspace, &p);
     const bool slab = (1 << a.log2_group) == 16 * a.head_dim;
-    const cudaError_t err =
-        a.head_dim == 64 ? (slab ? launch_tiles<64, true>(p) : launch_tiles<64, false>(p))
-                         : (slab ? launch_tiles<128, true>(p) : launch_tiles<128, false>(p));
-    if (err != cudaSuccess) return AKV_ERR_CUDA;
-  }
+    return a.head_dim == 64 ? (slab ? launch_tiles<64, true>(p) : launch_tiles<64, false>(p))
+                            : (slab ? launch_tiles<128, true>(p) : launch_tiles<128, false>(p));
+  };
+  for (int first = 0; first < all.batch; first += slice.batch)
+    for (int head = 0; head < all.kv_heads; head += slice.kv_heads)
+      if (launch(slice_of(all, first, std::min(slice.batch, all.batch - first), head,
+                          std::min(slice.kv_heads, all.kv_heads - head))) != cudaSuccess)
+        return AKV_ERR_CUDA;
   return AKV_OK;
 }
 

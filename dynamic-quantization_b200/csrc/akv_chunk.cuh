@@ -20,6 +20,7 @@ struct ChunkArgs {
   __half *out;
   int64_t o_bs, o_hs, o_ts;
   int32_t batch, rows, q_heads, kv_heads, head_dim, log2_group;
+  int32_t kv_first, page_heads;  // a call's slice has KV heads kv_first .. of the page_heads that pages hold
   int32_t window, sinks, lead;
   float scale;
   int32_t *status;
