@@ -20,7 +20,12 @@
 // kernel copies whole tiles.  It runs one CTA per SM, each with two row tiles that
 // share every K and V tile; the work (row tiles x tiles of tokens) is cut into equal
 // contiguous ranges, one per CTA, whose partial (O, m, l) a merge kernel joins.
-// Waits are bounded: a role whose wait runs out reports AKV_DEV_TIMEOUT and leaves.
+// Waits on mbarriers are bounded: a role whose wait runs out reports AKV_DEV_TIMEOUT and
+// leaves.  The named barrier of a row's two warps is not; a leaving warp arrives there
+// once, which is enough: its partner meets it at most once more before it waits on an
+// mbarrier that this warp's missing arrival (p_full or q_full) keeps from completing,
+// and leaves in turn.  A form in which a warp passes two exchanges without such a wait
+// between them would need more.
 //
 // What bounds it, measured on a B200 with clocks read in the kernel: a tile of tokens
 // takes about 3500 to 3700 clocks.  Of these a row tile's warps spend 150 on reading S,
@@ -28,8 +33,9 @@
 // special-function unit did nothing else) and 150 on handing P over; its next S is
 // there 1300 (head_dim 64) to 1700 clocks (128) later, behind O += P V, while the other
 // row tile is at its exponentials.  A 2048-token chunk of 32768 (32 heads over 8, 128)
-// takes 905 us, 1.1 PFLOP/s; 1000 tokens through a window of
-// 2048 (4 sequences, 24 heads over 8, 64) 150 us, of which the tiles take 115.
+// takes 905 us by itself, 1.1 PFLOP/s, and 1066 to 1097 in long runs, where the power
+// cap lowers the clock; 1000 tokens through a window of 2048
+// (4 sequences, 24 heads over 8, 64) 150 us, of which the tiles take 115.
 // Slower or no faster were: tiles of 64 tokens with S twice; S a tile ahead of P where
 // head_dim 64 leaves TMEM for it (149 to 157 us against 154); a thread per row tile
 // issuing the MMAs (1296 against 905); exponentials of some pairs by a polynomial
@@ -988,7 +994,9 @@ static int device_sms() {
 }
 
 // Raise a kernel's shared-memory limit, once per device, and check that it starts
-// with the registers its warpgroups then share out.
+// with the registers its warpgroups then share out: with fewer, setmaxnreg would wait
+// for ever.  A compiler that gives it another number makes every large chunk fail here
+// (AKV_ERR_CUDA) until kTileRegs and the split are set to its number.
 template <typename Kernel>
 static cudaError_t chunk_ready(Kernel kernel, int smem, int regs, std::atomic<bool> (&ready)[256]) {
   int dev = 0;

@@ -1802,19 +1802,23 @@ static int chunk_plan(int batch, int rows, int q_heads, int kv_heads, int head_d
 //   P 2048    INT4  g 16: 44, 54    g 32: 63, 65     FP16  g 16: 55, 53    g 32: 83, 63
 //   P 16384   INT4  g 8: 100, 122   g 12: 136, 125   FP16  g 6: 128, 115   g 8: 161, 118
 //   P 65536   INT4  g 8: 321, 340   g 12: 470, 345   FP16  g 4: 359, 318   g 8: 668, 322
-// The host does not know the pages' precisions, so the border lies between theirs.
+// The host does not know the pages' precisions, so the border lies between theirs.  It was
+// measured at this head_dim and head count alone, and both forms are far from the pages'
+// bytes there (P 16384: 5 us of INT4, 20 of FP16; 65536: 21 and 82): a chunk of one
+// block of 256 rows uses each unpacked tile once.
 static bool use_tiles(const ChunkPlan &c, int batch, int kv_heads) {
   const int64_t pages = (int64_t)batch * kv_heads * c.columns, groups = (c.rows_total / kv_heads + 7) / 8;
   return pages * (groups - 6) > 40000;
 }
 // Warps of a CTA that takes a whole item and writes its outputs, without a merge
 // kernel: as many as let every item have a CTA at once.  0: the items are too many or
-// too long for it.  Measured on a B200 against equal ranges and a merge (us, cold
+// too long for it.  Measured on a B200 beside equal ranges and a merge (us, cold
 // cache, INT4, 16 heads over 8 of 128; fill: the items' warps over those that fit):
-//   8 pages a warp     fill 0.05: 22.5 against 18.4   0.65: 34.8, 20.5   0.97: 36.9, 22.5
-//   16 pages a warp    fill 0.22: 24.6 against 28.7   0.54: 32.8, 30.7   0.97: 47.1, 32.8
-//   32 pages a warp    fill 0.65: 51.2 against 51.2   0.86: 55.3, 53.2   0.97: 67.6, 53.2
-//   64 pages a warp    fill 0.86: 92.2 against 98.3   0.97: 104.4, 98.3
+//                      equal ranges and a merge, then a CTA per item
+//   8 pages a warp     fill 0.05: 22.5, 18.4   0.65: 34.8, 20.5    0.97: 36.9, 22.5
+//   16 pages a warp    fill 0.22: 24.6, 28.7   0.54: 32.8, 30.7    0.97: 47.1, 32.8
+//   32 pages a warp    fill 0.65: 51.2, 51.2   0.86: 55.3, 53.2    0.97: 67.6, 53.2
+//   64 pages a warp    fill 0.86: 92.2, 98.3   0.97: 104.4, 98.3
 static int own_items(const ChunkPlan &c, int batch, int kv_heads) {
   constexpr int kDevice = 148 * DecodeTraits<128>::kMaxWarps;
   const int64_t items = (int64_t)batch * kv_heads * ((c.rows_total / kv_heads + 7) / 8);
