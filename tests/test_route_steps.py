@@ -202,3 +202,53 @@ def test_a_token_per_sequence_comes_in_any_shape(launches, shape, rows):
     assert given["ids"].tolist() == tokens.reshape(3, rows).tolist()
     assert given["at"].tolist() == list(range(20, 20 + rows)) and given["keep"] == rows
     assert out.shape == ((3, 5) if rows == 1 else (3, rows, 5))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,group,archive,recent,protected", [
+    (128, 64, 4, 1, (1,)), (64, 32, 8, 2, ()), (128, 128, 16, 2, ()), (64, 64, 4, 0, (0, 5))])
+def test_steps_with_forks_crops_and_compaction(cuda, dim, group, archive, recent, protected):
+    """Pages that wait for the archive are shared, reopened, copied and moved like others; every step is
+    checked against the token histories."""
+    from test_gpu_store import LAYERS as STORE_LAYERS
+    from test_gpu_store import _Histories
+
+    class Steps(_Histories):
+        def step(self, n):
+            ids, before = self._new(n), len(self.tokens[0])
+            for layer in range(STORE_LAYERS):
+                self.store.append(layer, *self._kv(ids, layer), archive=False)
+            self.tokens = [t + i.tolist() for t, i in zip(self.tokens, ids)]
+            self.old = max(self.old, before // 16 - self.recent - 1)
+            self.check()
+
+    h = Steps(cuda, dim, group, archive, recent, protected)
+    h.prefill(30)
+    h.step(37)                     # 67 tokens: pages 1 to 3 wait
+    h.attend(37)
+    h.fork([0, 1, 0, 0])           # waiting pages are shared
+    h.check()
+    h.crop(50)                     # into one that three sequences share
+    h.check()
+    h.step(5)
+    h.attend(5, window=20, sinks=3)
+    h.fork([2, 2, 1])
+    h.step(40)                     # shared pages archived once
+    h.crop(58)                     # back to what the step before wrote
+    h.check()
+    h.store.compact()
+    h.check()
+    h.step(60)
+    h.store.compact()              # with pages that wait
+    h.check()
+    h.attend(60, window=64)
+    h.append(1)                    # a single token archives at once
+    h.check()
+    h.step(3)
+    h.append(40)
+    h.check()
+    h.attend(3)
+    h.crop(0)
+    h.check()
+    h.step(20)
+    h.attend(20)
